@@ -51,6 +51,11 @@ extern "C" {
 #define VITB200_EPI_BIAS_GELU 2 /* Y = gelu_erf(acc + bias)                         */
 #define VITB200_EPI_BIAS_RESID 3/* Y = residual + acc + bias (residual may alias Y) */
 
+/* Element types of the operators below that take more than fp32. */
+#define VITB200_F32 0
+#define VITB200_F16 1
+#define VITB200_BF16 2
+
 /* ---- library / device management -------------------------------------- */
 
 /* Library version as 10000*major + 100*minor + patch. */
@@ -287,6 +292,40 @@ size_t vitb200_classifier_workspace_bytes(int B, int E, int C);
 int vitb200_classifier(const float* X, const float* W, const float* bias,
                        float* logits, int B, int T, int E, int C, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* ---- FP8 operators ------------------------------------------------------
+ * e4m3 codes with one fp32 scale per block of 128 columns of one row
+ * (activations) or per 128 x 128 block (weights); a value is code * scale. The
+ * last block of a row or column may be smaller. No counterpart in the
+ * reference. */
+
+/* Quantises x[rows][K] (x_type, row stride ldx elements): per block a =
+ * max|x|, scale = a / 448, code = e4m3(448 * x / a), each quotient rounded
+ * once; a below 1e-30 counts as 1e-30. A block with a NaN becomes NaN as a
+ * whole, one with an infinity dequantises to NaN. block_rows: 1, or 128 for
+ * weights. q[rows][ldq] (ldq >= K, ldq % 16 == 0, q 16-byte aligned; columns
+ * from K on are unspecified), scales[ceil(rows / block_rows)][ceil(K / 128)].
+ * K >= 1. */
+int vitb200_quantize_fp8(const void* x, int x_type, int64_t rows, int K, int64_t ldx,
+                         int block_rows, uint8_t* q, int64_t ldq, float* scales, void* stream);
+
+/* vitb200_layernorm's result (biased variance, affine) quantised with 1 x 128
+ * blocks, without ever storing it. gamma, beta: [K] fp32. */
+int vitb200_layernorm_fp8(const void* x, int x_type, int64_t rows, int K, int64_t ldx,
+                          const float* gamma, const float* beta, float eps, uint8_t* q,
+                          int64_t ldq, float* scales, void* stream);
+
+/* out[M][N] = residual + act(X W^T + bias): X[M][K] codes (row stride ldx
+ * bytes) with x_scales[M][ceil(K / 128)] (row stride ldxs), W[N][K] codes (ldw)
+ * with w_scales[ceil(N / 128)][ceil(K / 128)] (ldws). Products are summed in
+ * fp32 per block of 128 and the blocks in fp32 registers; bias (fp32), GELU
+ * (gelu != 0) and residual are optional; residual and out are out_type with row
+ * strides ldr and ldo elements (residual may alias out). ldx % 16 == 0,
+ * ldw % 16 == 0, X and W 16-byte aligned, K >= 1. */
+int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64_t ldxs,
+                     const uint8_t* W, int64_t ldw, const float* w_scales, int64_t ldws,
+                     const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
+                     int out_type, int64_t M, int K, int N, int gelu, void* stream);
 
 /* ---- whole-model forward (reference: vit_cuda/model.py:93-126) --------- */
 

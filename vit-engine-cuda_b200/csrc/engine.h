@@ -85,7 +85,8 @@ struct GemmProblem {
 int encode_tmap(CUtensorMap* map, int rank, const void* base, const uint64_t* dims,
                 const uint64_t* strides, const uint32_t* box, int swizzle128);
 
-// Same with FP16 elements when f16 != 0.
+// Same with 16-bit elements when f16 == 1 (a copy moves bits: bf16 too), bytes
+// when f16 == 2.
 int encode_tmap_typed(CUtensorMap* map, int rank, const void* base, const uint64_t* dims,
                       const uint64_t* strides, const uint32_t* box, int swizzle128, int f16);
 
@@ -180,6 +181,28 @@ int split_transpose_v_f16_launch(const float* v, int64_t ldv, int B, int T, int 
 // V[B*T][ldv] (head h at columns h*64..) -> vt pair [2][B*heads][64][T4].
 int split_transpose_v_launch(const float* v, int64_t ldv, int B, int T, int heads, float* vt_pair,
                              cudaStream_t s);
+
+// FP8 operators (quantize_fp8.cu, gemm_fp8.cu). Element types are VITB200_F32 /
+// _F16 / _BF16; codes are e4m3 bytes, scales one fp32 per block of 128.
+int quantize_fp8_launch(const void* x, int type, int64_t rows, int K, int64_t ldx, int block_rows,
+                        uint8_t* q, int64_t ldq, float* scales, cudaStream_t s);
+int layernorm_fp8_launch(const void* x, int type, int64_t rows, int K, int64_t ldx,
+                         const float* gamma, const float* beta, float eps, uint8_t* q, int64_t ldq,
+                         float* scales, cudaStream_t s);
+struct Fp8GemmProblem {
+  const uint8_t* x;       // [M][K] codes, rows ldx bytes apart
+  const uint8_t* w;       // [N][K] codes, rows ldw bytes apart
+  const float* xs;        // [M][ceil(K / 128)], rows ldxs apart
+  const float* ws;        // [ceil(N / 128)][ceil(K / 128)], rows ldws apart
+  const float* bias;      // [N] or null
+  const void* residual;   // [M][N] of out_type or null, rows ldr apart
+  void* out;              // [M][N] of out_type, rows ldo apart
+  int64_t M, ldx, ldw, ldxs, ldws, ldr, ldo;
+  int N, K, gelu, out_type;
+};
+int gemm_fp8_launch(const Fp8GemmProblem& p, cudaStream_t s);
+// Raises shared-memory limits of the FP8 GEMM kernels on the current device.
+int gemm_fp8_prepare_device();
 
 // Counts one kernel launch issued by the library (process-wide).
 void count_launch();

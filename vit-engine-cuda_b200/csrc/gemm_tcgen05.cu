@@ -1126,7 +1126,9 @@ int encode_tmap_typed(CUtensorMap* map, int rank, const void* base, const uint64
     if (i + 1 < rank) st[i] = static_cast<cuuint64_t>(strides[i]);
   }
   const CUtensorMapSwizzle sw = swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
-  const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+  const CUtensorMapDataType dt = f16 == 2   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                 : f16 != 0 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   CUresult r = enc(map, dt, static_cast<cuuint32_t>(rank),
                    const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -30,6 +30,11 @@ EPI_BIAS = 1
 EPI_BIAS_GELU = 2
 EPI_BIAS_RESID = 3
 
+# Element types of the operators that take more than fp32.
+F32 = 0
+F16 = 1
+BF16 = 2
+
 
 class VitB200Error(RuntimeError):
     """A libvitb200 entry point returned a non-zero status."""
@@ -112,6 +117,12 @@ _SIGNATURES = {
     "vitb200_classifier_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "vitb200_classifier": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, c_size_t,
                                    _P]),
+    "vitb200_quantize_fp8": (c_int, [_P, c_int, c_int64, c_int, c_int64, c_int, _P, c_int64, _P,
+                                     _P]),
+    "vitb200_layernorm_fp8": (c_int, [_P, c_int, c_int64, c_int, c_int64, _P, _P, c_float, _P,
+                                      c_int64, _P, _P]),
+    "vitb200_gemm_fp8": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P,
+                                 c_int64, _P, c_int64, c_int, c_int64, c_int, c_int, c_int, _P]),
     "vitb200_vit_workspace_bytes": (c_size_t, [POINTER(VitParams), c_int]),
     "vitb200_vit_forward": (c_int, [POINTER(VitParams), _P, _P, c_int, _P, c_size_t, _P]),
     "vitb200_vit_forward_features": (c_int, [POINTER(VitParams), _P, _P, c_int, _P, c_size_t,

@@ -23,7 +23,7 @@ from typing import Optional
 
 import torch
 
-from . import _C
+from . import _C, serving
 
 
 # ---------------------------------------------------------------- ops
@@ -115,6 +115,53 @@ def _(X, W, B):
     return X.new_empty((*X.shape[:-1], W.shape[0]))
 
 
+# ---------------------------------------------------------------- serving ops
+# vit_cuda.<op> calls these only while torch.compile traces; an eager call goes
+# straight to vit_cuda.serving, without the dispatcher's tens of microseconds,
+# which a single token's step would feel.
+def _fake_codes(X):
+    K = X.shape[-1]
+    ld = (K + 15) // 16 * 16
+    q = X.new_empty((*X.shape[:-1], ld), dtype=serving.FP8)
+    return q if ld == K else q[..., :K]
+
+
+@torch.library.custom_op("vit_cuda::quantize_fp8", mutates_args=())
+def _quantize_fp8(X: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return serving.quantize_fp8(X, block_rows)
+
+
+@_quantize_fp8.register_fake
+def _(X, block_rows):
+    kb = (X.shape[-1] + 127) // 128
+    lead = X.shape[:-1] if block_rows == 1 else ((X.shape[0] + 127) // 128,)
+    return _fake_codes(X), X.new_empty((*lead, kb), dtype=torch.float32)
+
+
+@torch.library.custom_op("vit_cuda::layernorm_fp8", mutates_args=())
+def _layernorm_fp8(X: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
+                   eps: float) -> tuple[torch.Tensor, torch.Tensor]:
+    return serving.layernorm_fp8(X, gamma, beta, eps)
+
+
+@_layernorm_fp8.register_fake
+def _(X, gamma, beta, eps):
+    kb = (X.shape[-1] + 127) // 128
+    return _fake_codes(X), X.new_empty((*X.shape[:-1], kb), dtype=torch.float32)
+
+
+@torch.library.custom_op("vit_cuda::gemm_fp8", mutates_args=())
+def _gemm_fp8(X: torch.Tensor, X_scale: torch.Tensor, W: torch.Tensor, W_scale: torch.Tensor,
+              B: Optional[torch.Tensor], residual: Optional[torch.Tensor], gelu: bool,
+              out_dtype: torch.dtype) -> torch.Tensor:
+    return serving.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+
+
+@_gemm_fp8.register_fake
+def _(X, X_scale, W, W_scale, B, residual, gelu, out_dtype):
+    return X.new_empty((*X.shape[:-1], W.shape[0]), dtype=out_dtype)
+
+
 # ---------------------------------------------------------------- whole model
 _MODELS: "weakref.WeakValueDictionary[int, object]" = weakref.WeakValueDictionary()
 _NEXT_ID = [0]
@@ -172,3 +219,25 @@ def qkv_proj(X, W, B):
 
 def gemm_bias(X, W, B):
     return torch.ops.vit_cuda.gemm_bias(X, W, B)
+
+
+def quantize_fp8(X, block_rows=1):
+    if torch.compiler.is_compiling():
+        return torch.ops.vit_cuda.quantize_fp8(X, block_rows)
+    return serving.quantize_fp8(X, block_rows)
+
+
+def layernorm_fp8(X, gamma, beta, eps):
+    if torch.compiler.is_compiling():
+        return torch.ops.vit_cuda.layernorm_fp8(X, gamma, beta, eps)
+    return serving.layernorm_fp8(X, gamma, beta, eps)
+
+
+def gemm_fp8(X, X_scale, W, W_scale, B=None, residual=None, gelu=False, out_dtype=torch.float32):
+    if torch.compiler.is_compiling():
+        return torch.ops.vit_cuda.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+    return serving.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+
+
+for _name in ("quantize_fp8", "layernorm_fp8", "gemm_fp8"):
+    globals()[_name].__doc__ = getattr(serving, _name).__doc__
