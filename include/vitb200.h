@@ -327,6 +327,25 @@ int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64
                      const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
                      int out_type, int64_t M, int K, int N, int gelu, void* stream);
 
+/* ---- cross attention ---------------------------------------------------- */
+
+/* softmax(Q K^T * scale) V of Tq queries over Tk keys of other states:
+ * q[B][Tq][heads * head_dim], k and v [B][Tk][kv_heads * head_dim] (type
+ * VITB200_F16 or _BF16, head_dim 64 or 128, heads a multiple of kv_heads: query
+ * head h attends to key head h / (heads / kv_heads)), o[B][Tq][heads *
+ * head_dim] contiguous. *_row and *_batch: elements between rows and between
+ * images (multiples of 8; pointers 16-byte aligned), so k and v may be column
+ * ranges of one projection's output. kv_lens: B int32 on the device, the keys of
+ * each image (clamped to 0..Tk), or NULL for Tk everywhere; keys past it are not
+ * read into the result, whatever they hold. An image without keys gets zeros.
+ * Scores, exponentials' sums and outputs are fp32, probabilities are rounded to
+ * `type` for the product with V, o is rounded once. No workspace. No counterpart
+ * in the reference (its attention has equal lengths, one type, 12 heads of 64). */
+int vitb200_cross_attention(const void* q, const void* k, const void* v, void* o, int type, int B,
+                            int Tq, int Tk, int heads, int kv_heads, int head_dim, int64_t q_row,
+                            int64_t q_batch, int64_t k_row, int64_t k_batch, int64_t v_row,
+                            int64_t v_batch, const int* kv_lens, float scale, void* stream);
+
 /* ---- whole-model forward (reference: vit_cuda/model.py:93-126) --------- */
 
 typedef struct vitb200_block_params {

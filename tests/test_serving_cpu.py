@@ -55,10 +55,31 @@ def test_gemm_status():
     assert gemm(N=0, out=None) == _lib.OK
 
 
+def cross(q=P, k=P, v=P, o=P, type=1, B=2, Tq=3, Tk=5, heads=4, kv_heads=2, D=64, qs=(256, 768),
+          ks=(128, 640), vs=(128, 640), lens=None):
+    return lib.vitb200_cross_attention(q, k, v, o, type, B, Tq, Tk, heads, kv_heads, D, *qs, *ks,
+                                       *vs, lens, 0.125, None)
+
+
+def test_cross_attention_status():
+    for kw in (dict(type=0), dict(type=3), dict(B=-1), dict(Tq=-1), dict(Tk=-1), dict(heads=0),
+               dict(kv_heads=0), dict(kv_heads=3), dict(q=None), dict(k=None), dict(v=None),
+               dict(o=None), dict(qs=(255, 768)), dict(ks=(64, 640)), dict(vs=(64, 640)),
+               dict(ks=(128, -8))):
+        assert cross(**kw) == _lib.E_INVALID_ARG, kw
+    for kw in (dict(q=P + 8), dict(k=P + 2), dict(v=P + 4), dict(o=P + 8), dict(qs=(260, 780)),
+               dict(ks=(132, 640)), dict(vs=(128, 644)), dict(lens=P + 2)):
+        assert cross(**kw) == _lib.E_ALIGNMENT, kw
+    assert cross(D=32) == cross(D=96) == _lib.E_UNSUPPORTED
+    assert cross(B=0, q=None) == _lib.OK
+    assert cross(Tq=0, o=None) == _lib.OK
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.randn(4, 128)
     q, s = x.to(torch.float8_e4m3fn), torch.ones(4, 1)
     for call in (lambda: vit_cuda.quantize_fp8(x), lambda: vit_cuda.gemm_fp8(q, s, q, s[:1]),
-                 lambda: vit_cuda.layernorm_fp8(x, x[0], x[0], 1e-6)):
+                 lambda: vit_cuda.layernorm_fp8(x, x[0], x[0], 1e-6),
+                 lambda: vit_cuda.cross_attention(x[None], x[None], x[None], 0.1, 2)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()

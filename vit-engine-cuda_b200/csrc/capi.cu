@@ -52,6 +52,7 @@ DeviceState* device_state(int* status) {
       if (!st) st = attention_prepare_device();
       if (!st) st = attention_f16_prepare_device();
       if (!st) st = gemm_fp8_prepare_device();
+      if (!st) st = cross_attention_prepare_device();
       if (st) d.ready = false;
     }
     d.status = st;

@@ -1,0 +1,718 @@
+// Attention of queries to an encoder's states of another length:
+//
+//   o[b][t][h] = softmax_s(q[b][t][h] . k[b][s][h / G] * scale) v[b][s][h / G]
+//
+// over keys s < len[b], bf16 or fp16, head size D = 64 or 128, G = heads /
+// kv_heads query heads to a key head. No key: o = 0.
+//
+// The rows a key head serves (G heads x Tq queries) are packed into tiles of up
+// to 128 rows, so a group of heads reads its keys once. A CTA runs two streams,
+// each with a softmax warpgroup (one row a thread), a score accumulator S and an
+// output accumulator O in TMEM:
+//  * two row tiles: both streams go over all key tiles and share the K and V
+//    copies;
+//  * one row tile: the streams take the even and the odd key tiles and their
+//    results are joined at the end.
+// Either way unit u = (stream u % 2, key tile) runs S = Q K^T, softmax, O += P V,
+// and while one stream's softmax runs the tensor core works for the other. P
+// overwrites S in TMEM as 16-bit pairs and is the A operand from there; V is the
+// N-major B operand as it lies in memory, no transposition.
+//
+// O stays in TMEM over all key tiles. With m the maximum that a row's
+// exponentials refer to, a new maximum within 2^8 of it leaves m as it is (P then
+// reaches at most 256, sums in fp32); only a larger one rescales O and the sum,
+// which after the first tiles is rare. The quotient o = O / l is the same.
+//
+// A launch with too few rows to fill the GPU shares the key tiles out over a
+// cluster of CTAs, joined in a fixed order through distributed shared memory: no
+// workspace, results independent of timing.
+// Every wait is bounded (device error word).
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <limits>
+#include <type_traits>
+
+#include "engine.h"
+#include "fp8.cuh"
+
+namespace vitb200 {
+
+namespace {
+
+constexpr int kRows = 128;       // rows of a tile
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kThreads = 384;    // control warpgroup + two softmax warpgroups
+// 384 threads launched at 168 registers: 128 * 56 + 256 * 224 = 384 * 168
+// (build.py checks that ptxas allocated 168).
+constexpr uint32_t kCtrlRegs = 56;
+constexpr uint32_t kSoftRegs = 224;
+static_assert(128 * kCtrlRegs + 256 * kSoftRegs == kThreads * 168, "register split");
+constexpr int kHalf = 64;                        // columns of one 128-byte swizzle span
+constexpr int kHalfBytes = kRows * kHalf * 2;    // 128 rows x 64 columns
+constexpr float kRescale = 8.f;                  // log2 of the largest P
+constexpr int kMaxSplit = 8;                     // portable cluster size
+
+template <int D>
+struct Cfg {
+  static constexpr int kHalves = D / kHalf;
+  static constexpr int kTile = kHalves * kHalfBytes;  // a Q, K or V tile
+  static constexpr int kKSlots = D == 64 ? 4 : 2;
+  static constexpr int kVSlots = D == 64 ? 4 : 3;
+  static constexpr int kSmem = (2 + kKSlots + kVSlots) * kTile + 1024;
+  // Partial results of both streams, joined at the end: [2][128][D + 4] floats
+  // (the pad keeps a thread-per-row store free of bank conflicts), then m and l.
+  static constexpr int kPitch = D + 4;
+  static constexpr int kStatsAt = 2 * kRows * kPitch;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static_assert((kStatsAt + 4 * kRows) * 4 <= kSmem - 1024, "partial results fit");
+};
+
+struct CrossArgs {
+  int Tq, Tk;
+  int kv_heads;    // key heads as the row tiles see them
+  int group;       // query heads packed into a row tile
+  int tile_t;      // queries per row tile (G * tile_t <= 128 rows)
+  int nq;          // row tiles per (image, key head)
+  int nsplit;      // CTAs per work item
+  int kv_div;      // packed key heads per key head (1 where groups are packed)
+  float c;         // scale * log2(e)
+  const int* lens; // [B] or null
+  uint16_t* o;     // [B][Tq][heads * D]
+  int64_t o_row;   // heads * D
+  int* err;
+};
+
+// S and P V instruction descriptors: fp32 accumulator, A and B f16 (0) or bf16
+// (1); V is N-major (bit 16).
+template <typename T>
+constexpr uint32_t idesc(int N, bool b_n_major) {
+  const uint32_t f = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  return make_idesc_f16(kRows, N) | (f << 7) | (f << 10) | (b_n_major ? 1u << 16 : 0u);
+}
+
+// N-major tile of [keys][64 columns] rows of 128 bytes under the 128-byte
+// swizzle: 8-key atoms 1024 bytes apart, the next 64 columns `halves` bytes on.
+__device__ __forceinline__ uint64_t sdesc_nmajor(uint32_t saddr, uint32_t half_bytes) {
+  return uint64_t((saddr >> 4) & 0x3FFFu) | (uint64_t(half_bytes >> 4) << 16) |
+         (uint64_t(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ bool warp_wait_x(uint64_t* bar, uint32_t parity, int* err, int code,
+                                            int lane) {
+  int ok = 1;
+  if (lane == 0) ok = mbar_wait(bar, parity, err, code) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+__device__ __forceinline__ void drain_wait_x(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t addr = smem_addr(bar);
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(addr, parity)) {
+    if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+      report_error(err, kErrDrain);
+      return;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Floats of a partial result, in this CTA's shared memory or a peer's.
+__device__ __forceinline__ float ld_partial(uint32_t addr, bool remote) {
+  float v;
+  if (remote)
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_partial4(uint32_t addr, bool remote) {
+  if (remote) return ld_shared_cluster_f4(addr);
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// A work item: a key head of an image and one or two of its row tiles.
+struct Item {
+  int b, hk, tile0, tiles;
+};
+__device__ __forceinline__ Item item_at(const CrossArgs& a, int i) {
+  const int groups = (a.nq + 1) / 2;
+  Item it;
+  const int bh = i / groups;
+  it.b = bh / a.kv_heads;
+  it.hk = bh - it.b * a.kv_heads;
+  it.tile0 = 2 * (i - bh * groups);
+  it.tiles = min(2, a.nq - it.tile0);
+  return it;
+}
+
+// Output row of packed row r of tile `tile`, or -1 past the last query.
+__device__ __forceinline__ int64_t out_row(const CrossArgs& a, const Item& it, int tile, int r,
+                                           int D) {
+  const int tl = r / a.group;
+  const int t = tile * a.tile_t + tl;
+  if (tl >= a.tile_t || t >= a.Tq) return -1;
+  return (static_cast<int64_t>(it.b) * a.Tq + t) * a.o_row +
+         (static_cast<int64_t>(it.hk) * a.group + (r - tl * a.group)) * D;
+}
+
+}  // namespace
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
+                           const __grid_constant__ CUtensorMap tmap_k,
+                           const __grid_constant__ CUtensorMap tmap_v, const CrossArgs a) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t q_full;
+  __shared__ __align__(8) uint64_t k_full[C::kKSlots], k_empty[C::kKSlots];
+  __shared__ __align__(8) uint64_t v_full[C::kVSlots], v_empty[C::kVSlots];
+  __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t tail_go, tail_bar;
+  __shared__ __align__(8) uint64_t mma_done;
+  __shared__ uint32_t tmem_slot;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  int* err = a.err;
+  const uint32_t raw = smem_addr(smem_raw);
+  uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* sq = base;
+  uint8_t* sk = base + 2 * C::kTile;
+  uint8_t* sv = sk + C::kKSlots * C::kTile;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < C::kKSlots; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < C::kVSlots; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);  // one arrival per warp of the stream's warpgroup
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(&tail_go, 1);
+    mbar_init(&tail_bar, 1);
+    mbar_init(&mma_done, 1);
+    fence_barrier_init();
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int split = static_cast<int>(blockIdx.x) % a.nsplit;  // = rank in the cluster
+  const Item it = item_at(a, static_cast<int>(blockIdx.x) / a.nsplit);
+  int len = a.Tk;
+  if (a.lens != nullptr) len = max(0, min(a.Tk, __ldg(a.lens + it.b)));
+  // This CTA's key tiles [j0, j0 + nk) of the image's `all`.
+  const int all = (len + kKeys - 1) / kKeys;
+  const int j0 = static_cast<int>(static_cast<int64_t>(all) * split / a.nsplit);
+  const int nk = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.nsplit) - j0;
+  const bool shared_keys = it.tiles == 2;  // two row tiles: every key tile is two units
+  const int units = shared_keys ? 2 * nk : nk;
+  // V's rows past the last key, inside its tile, may hold anything: P is zero
+  // there, but zero times NaN is not. (Rows past Tk arrive as zeros.)
+  const int tail_keys = len - (all - 1) * kKeys;
+  const bool fix_tail = nk > 0 && j0 + nk == all && len < a.Tk && tail_keys < kKeys;
+
+  if (warp < 4) {
+    setmaxnreg_dec<kCtrlRegs>();
+    if (warp == 0 && lane == 0 && nk > 0) {
+      // -------------------------------------------------------------- TMA
+      mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(it.tiles * C::kHalves * a.group *
+                                                           a.tile_t * kHalf * 2));
+      for (int i = 0; i < it.tiles; ++i)
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_5d(sq + i * C::kTile + h * kHalfBytes, &tmap_q, &q_full, h * kHalf, 0,
+                      (it.tile0 + i) * a.tile_t, it.hk, it.b);
+      int k_issued = 0, v_issued = 0;
+      auto load = [&](uint8_t* ring, int slots, uint64_t* full, uint64_t* empty,
+                      const CUtensorMap* map, int j, int& issued) -> bool {
+        const int s = j % slots;
+        if (!mbar_wait(&empty[s], ((j / slots) & 1) ^ 1u, err, kErrWaitEmpty)) return false;
+        mbar_arrive_expect_tx(&full[s], C::kTile);
+        for (int h = 0; h < C::kHalves; ++h)
+          tma_load_4d(ring + s * C::kTile + h * kHalfBytes, map, &full[s], h * kHalf,
+                      (j0 + j) * kKeys, it.hk / a.kv_div, it.b);
+        ++issued;
+        return true;
+      };
+      // Order of use: K runs one tile ahead of V.
+      bool ok = load(sk, C::kKSlots, k_full, k_empty, &tmap_k, 0, k_issued);
+      for (int j = 0; j < nk && ok; ++j) {
+        if (j + 1 < nk) ok = load(sk, C::kKSlots, k_full, k_empty, &tmap_k, j + 1, k_issued);
+        if (ok) ok = load(sv, C::kVSlots, v_full, v_empty, &tmap_v, j, v_issued);
+      }
+      if (fix_tail) mbar_arrive(&tail_go);
+      // Every copy issued lands before the CTA can exit.
+      drain_wait_x(&q_full, 0, err);
+      for (int s = 0; s < C::kKSlots; ++s)
+        if (k_issued > s)
+          drain_wait_x(&k_full[s], ((k_issued - 1 - s) / C::kKSlots) & 1, err);
+      for (int s = 0; s < C::kVSlots; ++s)
+        if (v_issued > s)
+          drain_wait_x(&v_full[s], ((v_issued - 1 - s) / C::kVSlots) & 1, err);
+    } else if (warp == 1 && lane == 0 && nk > 0) {
+      // -------------------------------------------------------------- MMA
+      constexpr uint32_t kIdescS = idesc<T>(kKeys, false);
+      constexpr uint32_t kIdescPV = idesc<T>(D, true);
+      const uint32_t q0 = smem_addr(sq), k0 = smem_addr(sk), v0 = smem_addr(sv);
+      auto key_tile = [&](int u) { return shared_keys ? u >> 1 : u; };
+      auto issue_s = [&](int u) -> bool {
+        const int i = u & 1, j = key_tile(u), s = j % C::kKSlots;
+        if (!mbar_wait(&k_full[s], (j / C::kKSlots) & 1, err, kErrWaitFull)) return false;
+        tc_fence_after();
+        const uint32_t qa = q0 + (shared_keys ? i * C::kTile : 0);
+        const uint32_t ka = k0 + s * C::kTile;
+#pragma unroll
+        for (int h = 0; h < C::kHalves; ++h) {
+          const uint64_t dq = make_sdesc_kmajor(qa + h * kHalfBytes, 128);
+          const uint64_t dk = make_sdesc_kmajor(ka + h * kHalfBytes, 128);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 16 columns = 32 bytes = +2
+            umma_f16(tmem + i * kKeys, dq + 2 * kk, dk + 2 * kk, kIdescS, h + kk ? 1u : 0u);
+        }
+        umma_commit(&s_full[i]);
+        if (!shared_keys || i == 1) umma_commit(&k_empty[s]);  // the tile's last use
+        return true;
+      };
+      auto issue_pv = [&](int u) -> bool {
+        const int i = u & 1, n = u >> 1, j = key_tile(u), s = j % C::kVSlots;
+        if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull) ||
+            !mbar_wait(&v_full[s], (j / C::kVSlots) & 1, err, kErrWaitFull))
+          return false;
+        const bool last = j0 + j == all - 1;
+        if (last && fix_tail && !mbar_wait(&tail_bar, 0, err, kErrWaitFull)) return false;
+        tc_fence_after();
+        const uint32_t d = tmem + 2 * kKeys + i * D;
+        const uint32_t p = tmem + i * kKeys;
+        const uint64_t dv = sdesc_nmajor(v0 + s * C::kTile, kHalfBytes);
+        const int steps = last ? (tail_keys + 15) / 16 : kKeys / 16;
+        for (int kk = 0; kk < steps; ++kk)  // 16 keys: 2048 bytes of V, 8 columns of P
+          umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
+        umma_commit(&pv_done[i]);
+        if (!shared_keys || i == 1) umma_commit(&v_empty[s]);
+        return true;
+      };
+      bool ok = mbar_wait(&q_full, 0, err, kErrWaitFull);
+      // S(u + 2) overwrites P(u): it is issued after the product that reads P(u),
+      // and one thread's products run in order.
+      for (int u = 0; u < 2 && u < units && ok; ++u) ok = issue_s(u);
+      for (int u = 0; u < units && ok; ++u) {
+        ok = issue_pv(u);
+        if (ok && u + 2 < units) ok = issue_s(u + 2);
+      }
+      umma_commit(&mma_done);
+      drain_wait_x(&mma_done, 0, err);
+    } else if (warp == 2 && fix_tail) {
+      // ------------------------------------------------------------- tail
+      // Not before the copy is issued: until then the slot's barrier may be a
+      // whole turn of the ring behind, and its parity would say nothing.
+      const int j = nk - 1, s = j % C::kVSlots;
+      if (warp_wait_x(&tail_go, 0, err, kErrWaitFull, lane) &&
+          warp_wait_x(&v_full[s], (j / C::kVSlots) & 1, err, kErrWaitFull, lane)) {
+        uint4* v = reinterpret_cast<uint4*>(sv + s * C::kTile);
+        constexpr int kRow16 = 8;  // 16-byte chunks of a 128-byte row
+        for (int h = 0; h < C::kHalves; ++h)
+          for (int c = tail_keys * kRow16 + lane; c < kKeys * kRow16; c += 32)
+            v[h * (kHalfBytes / 16) + c] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tail_bar);
+      }
+    }
+    __syncwarp();
+  }
+
+  // Softmax state of this thread's row, kept past the role split.
+  const bool joined = a.nsplit > 1 || !shared_keys;  // rows have several partial results
+  if (warp >= 4) {
+    setmaxnreg_inc<kSoftRegs>();
+    // ---------------------------------------------------------------- softmax
+    const int i = (warp - 4) >> 2;  // stream
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t s_col = lanes + i * kKeys;
+    const uint32_t o_col = lanes + 2 * kKeys + i * D;
+    const int mine = (units + 1 - i) / 2;  // units of this stream
+    const float c = a.c;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int n = 0; n < mine; ++n) {
+      const int j = j0 + (shared_keys ? n : 2 * n + i);
+      if (!warp_wait_x(&s_full[i], n & 1, err, kErrWaitAccFull, lane)) {
+        ok = false;
+        break;
+      }
+      // S(n) was issued after the stream's product n - 1: that one is in O.
+      if (n > 0 && !warp_wait_x(&pv_done[i], (n - 1) & 1, err, kErrWaitAccFull, lane)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float s[kKeys];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float t[32];
+        tmem_ld_32x32b_x32(s_col + 32 * h, t);
+#pragma unroll
+        for (int x = 0; x < 32; ++x) s[32 * h + x] = t[x];
+      }
+      const int valid = len - j * kKeys;
+      if (valid < kKeys) {
+        const float out = c < 0.f ? INFINITY : -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kKeys; ++x)
+          if (x >= valid) s[x] = out;
+      }
+      // The largest s * c (the smallest s where c is negative).
+      float e0 = s[0], e1 = s[1], e2 = s[2], e3 = s[3];
+      if (c >= 0.f) {
+#pragma unroll
+        for (int x = 4; x < kKeys; x += 4) {
+          e0 = fmaxf(e0, s[x]), e1 = fmaxf(e1, s[x + 1]);
+          e2 = fmaxf(e2, s[x + 2]), e3 = fmaxf(e3, s[x + 3]);
+        }
+        e0 = fmaxf(fmaxf(e0, e1), fmaxf(e2, e3));
+      } else {
+#pragma unroll
+        for (int x = 4; x < kKeys; x += 4) {
+          e0 = fminf(e0, s[x]), e1 = fminf(e1, s[x + 1]);
+          e2 = fminf(e2, s[x + 2]), e3 = fminf(e3, s[x + 3]);
+        }
+        e0 = fminf(fminf(e0, e1), fminf(e2, e3));
+      }
+      const float top = e0 * c;
+      if (n == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, top > m + kRescale)) {
+        float f = 1.f;
+        if (top > m + kRescale) {
+          f = ex2_approx(m - top);
+          m = top;
+        }
+        l *= f;
+#pragma unroll 1
+        for (int h = 0; h < D; h += 32) {
+          float t[32];
+          tmem_ld_32x32b_x32(o_col + h, t);
+#pragma unroll
+          for (int x = 0; x < 32; ++x) t[x] *= f;
+          tmem_st_32x32b_x32(o_col + h, t);
+        }
+        tmem_wait_st();
+      }
+      // All scores -inf so far: 2^(-inf - 0) = 0, not NaN.
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const float p0 = ex2_approx(fmaf(s[64 * h + 2 * x], c, -ref));
+          const float p1 = ex2_approx(fmaf(s[64 * h + 2 * x + 1], c, -ref));
+          l0 += p0;
+          l1 += p1;
+          p[x] = __uint_as_float(pack2<T>(p0, p1));
+        }
+        tmem_st_32x32b_x32(s_col + 32 * h, p);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[i]);
+    }
+    if (ok && mine > 0)
+      ok = warp_wait_x(&pv_done[i], (mine - 1) & 1, err, kErrWaitAccFull, lane);
+    tc_fence_after();
+    if (ok && !joined) {
+      // Two row tiles, all keys here: this thread's row is complete.
+      const int64_t row = out_row(a, it, it.tile0 + i, r, D);
+      const float inv = 1.f / l;
+#pragma unroll 1
+      for (int h = 0; h < D; h += 32) {
+        float t[32];
+        if (len > 0) {
+          __syncwarp();
+          tmem_ld_32x32b_x32(o_col + h, t);
+        }
+        if (row >= 0) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (len > 0)
+              w = make_uint4(pack2<T>(t[x] * inv, t[x + 1] * inv),
+                             pack2<T>(t[x + 2] * inv, t[x + 3] * inv),
+                             pack2<T>(t[x + 4] * inv, t[x + 5] * inv),
+                             pack2<T>(t[x + 6] * inv, t[x + 7] * inv));
+            *reinterpret_cast<uint4*>(a.o + row + h + x) = w;
+          }
+        }
+      }
+    } else if (ok) {
+      // Leave the partial result in shared memory: this stream's products have
+      // read the tiles there, the other's may not have, so wait for it too. A
+      // stream without units leaves an empty result.
+      const int theirs = (units + i) / 2;
+      if (theirs > 0)
+        ok = warp_wait_x(&pv_done[1 - i], (theirs - 1) & 1, err, kErrWaitAccFull, lane);
+      if (ok) {
+        fence_proxy_async_smem();
+        float* part = reinterpret_cast<float*>(base);
+        float* mine_at = part + (i * kRows + r) * C::kPitch;
+#pragma unroll 1
+        for (int h = 0; h < D; h += 32) {
+          float t[32];
+          if (mine > 0) {
+            __syncwarp();
+            tmem_ld_32x32b_x32(o_col + h, t);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) t[x] = 0.f;
+          }
+#pragma unroll
+          for (int x = 0; x < 32; x += 4)
+            *reinterpret_cast<float4*>(mine_at + h + x) =
+                make_float4(t[x], t[x + 1], t[x + 2], t[x + 3]);
+        }
+        part[C::kStatsAt + i * kRows + r] = m;
+        part[C::kStatsAt + 2 * kRows + i * kRows + r] = l;
+      }
+    }
+  }
+
+  tc_fence_before();
+  if (a.nsplit > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  if (!joined) return;
+
+  // Join the partial results (the softmax warps: the control warps gave their
+  // registers up), eight columns a thread, the rows shared out over
+  // the cluster: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p. Row tile i of
+  // two has one result per CTA (stream i); a single row tile has two.
+  const int streams = shared_keys ? 1 : 2;
+  constexpr int kChunks = D / 8;
+  const uint32_t part = smem_addr(base);
+  constexpr int kJoiners = kThreads - 128;
+  for (int x = split * kJoiners + static_cast<int>(threadIdx.x) - 128;
+       warp >= 4 && x < it.tiles * kRows * kChunks; x += a.nsplit * kJoiners) {
+    const int col = 8 * (x % kChunks);
+    const int tr = x / kChunks;
+    const int tile = tr / kRows, r = tr - tile * kRows;
+    const int64_t row = out_row(a, it, it.tile0 + tile, r, D);
+    if (row < 0) continue;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (len > 0) {
+      auto peer = [&](int p, int at) {  // float `at` of partial result p's CTA
+        const uint32_t addr = part + static_cast<uint32_t>(at) * 4u;
+        return a.nsplit > 1 ? mapa_shared(addr, static_cast<uint32_t>(p / streams)) : addr;
+      };
+      auto slot = [&](int p) { return (shared_keys ? tile : p % streams) * kRows + r; };
+      const int parts = a.nsplit * streams;
+      float M = -INFINITY;
+      for (int p = 0; p < parts; ++p)
+        M = fmaxf(M, ld_partial(peer(p, C::kStatsAt + slot(p)), a.nsplit > 1));
+      if (M == -INFINITY) M = 0.f;
+      float L = 0.f, o[8] = {};
+      for (int p = 0; p < parts; ++p) {
+        const float f = ex2_approx(ld_partial(peer(p, C::kStatsAt + slot(p)), a.nsplit > 1) - M);
+        L = fmaf(ld_partial(peer(p, C::kStatsAt + 2 * kRows + slot(p)), a.nsplit > 1), f, L);
+#pragma unroll
+        for (int q = 0; q < 8; q += 4) {
+          const float4 t =
+              ld_partial4(peer(p, slot(p) * C::kPitch + col + q), a.nsplit > 1);
+          o[q] = fmaf(t.x, f, o[q]), o[q + 1] = fmaf(t.y, f, o[q + 1]);
+          o[q + 2] = fmaf(t.z, f, o[q + 2]), o[q + 3] = fmaf(t.w, f, o[q + 3]);
+        }
+      }
+      const float inv = 1.f / L;
+      w = make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                     pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
+    }
+    *reinterpret_cast<uint4*>(a.o + row + col) = w;
+  }
+  __syncwarp();
+  if (a.nsplit > 1) cluster_sync_all();  // no CTA exits while its results may be read
+}
+
+// ---------------------------------------------------------------- host side
+namespace {
+
+template <typename T, int D>
+int launch_tiles(const CrossProblem& p, cudaStream_t s) {
+  using C = Cfg<D>;
+  CrossArgs a = {};
+  const int G = p.heads / p.kv_heads;
+  a.Tq = p.Tq;
+  a.Tk = p.Tk;
+  a.lens = p.lens;
+  a.o = static_cast<uint16_t*>(p.o);
+  a.o_row = static_cast<int64_t>(p.heads) * D;
+  a.c = p.scale * 1.44269504088896340736f;  // log2(e)
+  // Masked scores are infinite, and infinity times zero is NaN: the smallest
+  // float instead moves no score by more than 5e-7.
+  if (a.c == 0.f) a.c = std::numeric_limits<float>::denorm_min();
+  a.err = device_error_word();
+  // Pack a key head's G query heads into its row tiles; groups too large for a
+  // tile (or that would waste half of one) run head by head, every query head
+  // with its own copy of the key head.
+  const bool pack = G <= kRows / 2 || kRows % G == 0;
+  a.group = pack ? G : 1;
+  a.kv_heads = pack ? p.kv_heads : p.heads;
+  a.tile_t = std::min(kRows / a.group, p.Tq);
+  a.nq = (p.Tq + a.tile_t - 1) / a.tile_t;
+  const int64_t items = static_cast<int64_t>(p.B) * a.kv_heads * ((a.nq + 1) / 2);
+  if (items > INT32_MAX / kMaxSplit) return VITB200_E_UNSUPPORTED;
+  const int key_tiles = std::max(1, (p.Tk + kKeys - 1) / kKeys);
+  a.nsplit = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>({device_num_sms() / items, key_tiles, kMaxSplit})));
+
+  CUtensorMap tq, tk, tv;
+  const uint64_t es = 2;
+  {
+    const uint64_t dims[5] = {D, static_cast<uint64_t>(a.group), static_cast<uint64_t>(p.Tq),
+                              static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(p.B)};
+    const uint64_t strides[4] = {D * es, static_cast<uint64_t>(p.q_row) * es,
+                                 static_cast<uint64_t>(a.group) * D * es,
+                                 static_cast<uint64_t>(p.q_batch) * es};
+    const uint32_t box[5] = {kHalf, static_cast<uint32_t>(a.group),
+                             static_cast<uint32_t>(a.tile_t), 1, 1};
+    if (int st = encode_tmap_typed(&tq, 5, p.q, dims, strides, box, 1, 1)) return st;
+  }
+  auto kv_map = [&](CUtensorMap* map, const void* t, int64_t row, int64_t batch) {
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(p.Tk), static_cast<uint64_t>(p.kv_heads),
+                              static_cast<uint64_t>(p.B)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(row) * es, D * es,
+                                 static_cast<uint64_t>(batch) * es};
+    const uint32_t box[4] = {kHalf, kKeys, 1, 1};
+    return encode_tmap_typed(map, 4, t, dims, strides, box, 1, 1);
+  };
+  if (int st = kv_map(&tk, p.k, p.k_row, p.k_batch)) return st;
+  if (int st = kv_map(&tv, p.v, p.v_row, p.v_batch)) return st;
+  a.kv_div = p.heads / p.kv_heads / a.group;
+  return launch_kernel(cross_attention_kernel<T, D>,
+                       dim3(static_cast<unsigned>(items * a.nsplit)), dim3(kThreads), C::kSmem, s,
+                       static_cast<unsigned>(a.nsplit), tq, tk, tv, a);
+}
+
+template <typename F>
+int with_head(int type, int D, F&& f) {
+  auto typed = [&](auto tag) {
+    if (D == 64) return f(tag, std::integral_constant<int, 64>{});
+    return f(tag, std::integral_constant<int, 128>{});
+  };
+  return type == VITB200_BF16 ? typed(__nv_bfloat16{}) : typed(__half{});
+}
+
+}  // namespace
+
+int cross_attention_prepare_device() {
+  for (int type : {VITB200_F16, VITB200_BF16})
+    for (int D : {64, 128}) {
+      const int st = with_head(type, D, [](auto tag, auto d) {
+        return cuda_status(cudaFuncSetAttribute(cross_attention_kernel<decltype(tag), d.value>,
+                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                Cfg<d.value>::kSmem));
+      });
+      if (st) return st;
+    }
+  return 0;
+}
+
+int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
+  return with_head(p.type, p.D, [&](auto tag, auto d) {
+    return launch_tiles<decltype(tag), d.value>(p, s);
+  });
+}
+
+}  // namespace vitb200
+
+using namespace vitb200;
+
+extern "C" int vitb200_cross_attention(const void* q, const void* k, const void* v, void* o,
+                                       int type, int B, int Tq, int Tk, int heads, int kv_heads,
+                                       int head_dim, int64_t q_row, int64_t q_batch, int64_t k_row,
+                                       int64_t k_batch, int64_t v_row, int64_t v_batch,
+                                       const int* kv_lens, float scale, void* stream) {
+  try {
+    if (type != VITB200_F16 && type != VITB200_BF16) return VITB200_E_INVALID_ARG;
+    if (B < 0 || Tq < 0 || Tk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
+      return VITB200_E_INVALID_ARG;
+    if (head_dim != 64 && head_dim != 128) return VITB200_E_UNSUPPORTED;
+    if (Tq > INT32_MAX - 256 || Tk > INT32_MAX - 256 || heads > 65535) return VITB200_E_UNSUPPORTED;
+    const int64_t wq = static_cast<int64_t>(heads) * head_dim;
+    const int64_t wk = static_cast<int64_t>(kv_heads) * head_dim;
+    if (q_row < wq || k_row < wk || v_row < wk || q_batch < 0 || k_batch < 0 || v_batch < 0)
+      return VITB200_E_INVALID_ARG;
+    if (B == 0 || Tq == 0) return 0;
+    if (!q || !o || (Tk > 0 && (!k || !v))) return VITB200_E_INVALID_ARG;
+    for (const void* t : {q, k, v, static_cast<const void*>(o)})
+      if (reinterpret_cast<uintptr_t>(t) % 16 != 0) return VITB200_E_ALIGNMENT;
+    for (int64_t st : {q_row, q_batch, k_row, k_batch, v_row, v_batch})
+      if (st % 8 != 0) return VITB200_E_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(kv_lens) % 4 != 0) return VITB200_E_ALIGNMENT;
+    if (int st = vitb200_init()) return st;
+    if (Tk == 0)
+      return cuda_status(cudaMemsetAsync(o, 0, static_cast<size_t>(B) * Tq * wq * 2,
+                                         static_cast<cudaStream_t>(stream)));
+    CrossProblem p = {};
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.o = o;
+    p.lens = kv_lens;
+    p.type = type;
+    p.B = B;
+    p.Tq = Tq;
+    p.Tk = Tk;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.D = head_dim;
+    p.q_row = q_row;
+    p.q_batch = q_batch;
+    p.k_row = k_row;
+    p.k_batch = k_batch;
+    p.v_row = v_row;
+    p.v_batch = v_batch;
+    p.scale = scale;
+    return cross_attention_launch(p, static_cast<cudaStream_t>(stream));
+  } catch (...) {
+    return VITB200_E_INVALID_ARG;
+  }
+}

@@ -204,6 +204,23 @@ int gemm_fp8_launch(const Fp8GemmProblem& p, cudaStream_t s);
 // Raises shared-memory limits of the FP8 GEMM kernels on the current device.
 int gemm_fp8_prepare_device();
 
+// Attention to states of another length (cross_attention.cu); strides in
+// elements. q [B][Tq][heads * D], k and v [B][Tk][kv_heads * D], o contiguous.
+struct CrossProblem {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  const int* lens;  // [B] keys per image, or null
+  int type;         // VITB200_F16 or _BF16
+  int B, Tq, Tk, heads, kv_heads, D;
+  int64_t q_row, q_batch, k_row, k_batch, v_row, v_batch;
+  float scale;
+};
+int cross_attention_launch(const CrossProblem& p, cudaStream_t s);
+// Raises shared-memory limits of its kernels on the current device.
+int cross_attention_prepare_device();
+
 // Counts one kernel launch issued by the library (process-wide).
 void count_launch();
 

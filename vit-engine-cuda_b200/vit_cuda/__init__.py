@@ -6,9 +6,9 @@ names go through ``torch.ops.vit_cuda.<op>`` (registered custom ops that
 ``torch.compile`` traces); ``vit_cuda._C.<op>`` calls the library directly.
 """
 from . import _C
-from .library import (classifier_forward, flash_attn_2, gemm_bias, gemm_fp8, layernorm_forward,
-                      layernorm_fp8, mlp_forward, patch_embed, pos_encoding, qkv_proj,
-                      quantize_fp8)
+from .library import (classifier_forward, cross_attention, flash_attn_2, gemm_bias, gemm_fp8,
+                      layernorm_forward, layernorm_fp8, mlp_forward, patch_embed, pos_encoding,
+                      qkv_proj, quantize_fp8)
 from ._lib import VitB200Error, device_error, set_split_k
 from .model import ViTBlockCUDA, ViTCUDA
 from .pipeline import StreamedInference
@@ -26,6 +26,7 @@ __all__ = [
     "quantize_fp8",
     "layernorm_fp8",
     "gemm_fp8",
+    "cross_attention",
     "ViTCUDA",
     "ViTBlockCUDA",
     "VitB200Error",

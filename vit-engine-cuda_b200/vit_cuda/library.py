@@ -162,6 +162,17 @@ def _(X, X_scale, W, W_scale, B, residual, gelu, out_dtype):
     return X.new_empty((*X.shape[:-1], W.shape[0]), dtype=out_dtype)
 
 
+@torch.library.custom_op("vit_cuda::cross_attention", mutates_args=())
+def _cross_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, scale: float, heads: int,
+                     kv_heads: Optional[int], kv_lens: Optional[torch.Tensor]) -> torch.Tensor:
+    return serving.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+
+
+@_cross_attention.register_fake
+def _(Q, K, V, scale, heads, kv_heads, kv_lens):
+    return Q.new_empty(Q.shape)
+
+
 # ---------------------------------------------------------------- whole model
 _MODELS: "weakref.WeakValueDictionary[int, object]" = weakref.WeakValueDictionary()
 _NEXT_ID = [0]
@@ -239,5 +250,11 @@ def gemm_fp8(X, X_scale, W, W_scale, B=None, residual=None, gelu=False, out_dtyp
     return serving.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
 
 
-for _name in ("quantize_fp8", "layernorm_fp8", "gemm_fp8"):
+def cross_attention(Q, K, V, scale, heads, kv_heads=None, kv_lens=None):
+    if torch.compiler.is_compiling():
+        return torch.ops.vit_cuda.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+    return serving.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+
+
+for _name in serving.__all__:
     globals()[_name].__doc__ = getattr(serving, _name).__doc__
