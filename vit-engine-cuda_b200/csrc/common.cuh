@@ -146,6 +146,63 @@ __device__ __forceinline__ float gelu_erf(float x) {
   return x > 0.f ? x - y : y;
 }
 
+// Two fp32 operations in one instruction, each rounded as its scalar form.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+// The largest of three (NaN loses, as with fmaxf).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 splat2(float v) { return make_float2(v, v); }
+
+// gelu_erf of two values with paired operations: the same polynomial, and
+// GELU(x) = max(x, 0) - |x| e for either sign of x.
+__device__ __forceinline__ float2 gelu_erf2(float2 x) {
+  const float2 a = make_float2(fminf(fabsf(x.x), 5.6f), fminf(fabsf(x.y), 5.6f));
+  float2 h = splat2(-1.648524517e-08f);
+  h = fma2(h, a, splat2(5.266558105e-07f));
+  h = fma2(h, a, splat2(-7.210927379e-06f));
+  h = fma2(h, a, splat2(5.323315054e-05f));
+  h = fma2(h, a, splat2(-1.941426890e-04f));
+  h = fma2(h, a, splat2(-1.917099726e-04f));
+  h = fma2(h, a, splat2(7.203671150e-03f));
+  h = fma2(h, a, splat2(-5.263466015e-02f));
+  h = fma2(h, a, splat2(2.621984780e-01f));
+  h = fma2(h, a, splat2(-1.151113629e+00f));
+  h = fma2(h, a, splat2(-1.f));
+  const float2 t = fma2(mul2(x, x), splat2(-0.72134752044448170368f), h);  // 1/(2 ln 2)
+  const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+  return fma2(make_float2(-fabsf(x.x), -fabsf(x.y)), e,
+              make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
+}
+
 // ---- shared memory / mbarrier -----------------------------------------
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -385,31 +442,56 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, float (&v)[16
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// The same load of 32 columns in two steps, so that other work can overlap it:
-// `issue` starts it, and the registers hold the columns after `wait`, which
-// waits for every load this warp has issued. `wait` names them as operands so
-// that no use can move above it.
-__device__ __forceinline__ void tmem_ld_issue_x32(uint32_t taddr, uint32_t (&r)[32]) {
+// The same load of 32 columns in two steps, so that other work (more loads, say)
+// can overlap it: `issue` starts it, and the registers hold the columns after
+// `wait`, which waits for every load this warp has issued. `wait` names them as
+// operands so that no use can move above it; `landed` does that for the
+// registers of further loads that a wait has covered.
+__device__ __forceinline__ void tmem_ld_issue_x32(uint32_t taddr, float* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
       "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+        "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]),
+        "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
+        "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]),
+        "=f"(r[31])
       : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait_x32(uint32_t (&r)[32]) {
+#define VITB200_LANDED_32(text, r)                                                             \
+  asm volatile(text                                                                            \
+               : "+f"((r)[0]), "+f"((r)[1]), "+f"((r)[2]), "+f"((r)[3]), "+f"((r)[4]),         \
+                 "+f"((r)[5]), "+f"((r)[6]), "+f"((r)[7]), "+f"((r)[8]), "+f"((r)[9]),         \
+                 "+f"((r)[10]), "+f"((r)[11]), "+f"((r)[12]), "+f"((r)[13]), "+f"((r)[14]),    \
+                 "+f"((r)[15]), "+f"((r)[16]), "+f"((r)[17]), "+f"((r)[18]), "+f"((r)[19]),    \
+                 "+f"((r)[20]), "+f"((r)[21]), "+f"((r)[22]), "+f"((r)[23]), "+f"((r)[24]),    \
+                 "+f"((r)[25]), "+f"((r)[26]), "+f"((r)[27]), "+f"((r)[28]), "+f"((r)[29]),    \
+                 "+f"((r)[30]), "+f"((r)[31])                                                  \
+               :                                                                               \
+               : "memory")
+__device__ __forceinline__ void tmem_ld_wait_x32(float* r) {
+  VITB200_LANDED_32("tcgen05.wait::ld.sync.aligned;", r);
+}
+__device__ __forceinline__ void tmem_ld_landed_x32(float* r) { VITB200_LANDED_32("", r); }
+#undef VITB200_LANDED_32
+
+// 16 columns.
+__device__ __forceinline__ void tmem_ld_issue_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait_x16(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
                  "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31])
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
 }
@@ -550,6 +632,13 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
+// Arrival that orders nothing but itself (and, after tcgen05.fence, this
+// thread's TMEM reads): a release at cluster scope waits for every memory access
+// in flight.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Bounded wait, with acquire at cluster scope, on a barrier of this CTA that
 // threads of other CTAs of the cluster arrive on (mbar_arrive_cluster): their
 // writes before the arrival are visible to this thread afterwards.
@@ -662,6 +751,15 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
           bar_cluster)
+      : "memory");
+}
+
+// The same, on the barrier at this shared::cta address in both CTAs at once.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_addr(bar)),
+      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 

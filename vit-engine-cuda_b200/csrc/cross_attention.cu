@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t q_full;
   __shared__ __align__(8) uint64_t k_full[C::kKSlots], k_empty[C::kKSlots];
   __shared__ __align__(8) uint64_t v_full[C::kVSlots], v_empty[C::kVSlots];
-  __shared__ __align__(8) uint64_t s_full[2], p_full[2], pv_done[2];
+  __shared__ __align__(8) uint64_t s_full[2], p_half[2], p_full[2], pv_done[2];
   __shared__ __align__(8) uint64_t tail_go, tail_bar;
   __shared__ __align__(8) uint64_t mma_done;
   __shared__ uint32_t tmem_slot;
@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::kVSlots; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);  // one arrival per warp of the stream's warpgroup
+      mbar_init(&p_half[i], 4);  // one arrival per warp of the stream's warpgroup
+      mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(&tail_go, 1);
@@ -305,18 +306,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto issue_pv = [&](int u) -> bool {
         const int i = u & 1, n = u >> 1, j = key_tile(u), s = j % C::kVSlots;
-        if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull) ||
-            !mbar_wait(&v_full[s], (j / C::kVSlots) & 1, err, kErrWaitFull))
-          return false;
+        if (!mbar_wait(&v_full[s], (j / C::kVSlots) & 1, err, kErrWaitFull)) return false;
         const bool last = j0 + j == all - 1;
         if (last && fix_tail && !mbar_wait(&tail_bar, 0, err, kErrWaitFull)) return false;
-        tc_fence_after();
         const uint32_t d = tmem + 2 * kKeys + i * D;
         const uint32_t p = tmem + i * kKeys;
         const uint64_t dv = sdesc_nmajor(v0 + s * C::kTile, kHalfBytes);
         const int steps = last ? (tail_keys + 15) / 16 : kKeys / 16;
-        for (int kk = 0; kk < steps; ++kk)  // 16 keys: 2048 bytes of V, 8 columns of P
+        // The first half of the keys while the exponentials of the second run.
+        if (!mbar_wait(&p_half[i], n & 1, err, kErrWaitAccFull)) return false;
+        tc_fence_after();
+        for (int kk = 0; kk < min(4, steps); ++kk)  // 16 keys: 2048 bytes of V, 8 columns of P
           umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
+        if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+        tc_fence_after();
+        for (int kk = 4; kk < steps; ++kk)
+          umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
         umma_commit(&pv_done[i]);
         if (!shared_keys || i == 1) umma_commit(&v_empty[s]);
         return true;
@@ -380,12 +385,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       float s[kKeys];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        float t[32];
-        tmem_ld_32x32b_x32(s_col + 32 * h, t);
+      for (int h = 0; h < 4; ++h) tmem_ld_issue_x32(s_col + 32 * h, s + 32 * h);
+      tmem_ld_wait_x32(s);
 #pragma unroll
-        for (int x = 0; x < 32; ++x) s[32 * h + x] = t[x];
-      }
+      for (int h = 1; h < 4; ++h) tmem_ld_landed_x32(s + 32 * h);
       const int valid = len - j * kKeys;
       if (valid < kKeys) {
         const float out = c < 0.f ? INFINITY : -INFINITY;
@@ -397,18 +400,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       float e0 = s[0], e1 = s[1], e2 = s[2], e3 = s[3];
       if (c >= 0.f) {
 #pragma unroll
-        for (int x = 4; x < kKeys; x += 4) {
-          e0 = fmaxf(e0, s[x]), e1 = fmaxf(e1, s[x + 1]);
-          e2 = fmaxf(e2, s[x + 2]), e3 = fmaxf(e3, s[x + 3]);
+        for (int x = 4; x + 8 <= kKeys; x += 8) {
+          e0 = max3(e0, s[x], s[x + 4]), e1 = max3(e1, s[x + 1], s[x + 5]);
+          e2 = max3(e2, s[x + 2], s[x + 6]), e3 = max3(e3, s[x + 3], s[x + 7]);
         }
-        e0 = fmaxf(fmaxf(e0, e1), fmaxf(e2, e3));
+        e0 = max3(e0, s[kKeys - 4], s[kKeys - 3]);
+        e1 = max3(e1, s[kKeys - 2], s[kKeys - 1]);
+        e0 = fmaxf(max3(e0, e1, e2), e3);
       } else {
 #pragma unroll
-        for (int x = 4; x < kKeys; x += 4) {
-          e0 = fminf(e0, s[x]), e1 = fminf(e1, s[x + 1]);
-          e2 = fminf(e2, s[x + 2]), e3 = fminf(e3, s[x + 3]);
+        for (int x = 4; x + 8 <= kKeys; x += 8) {
+          e0 = min3(e0, s[x], s[x + 4]), e1 = min3(e1, s[x + 1], s[x + 5]);
+          e2 = min3(e2, s[x + 2], s[x + 6]), e3 = min3(e3, s[x + 3], s[x + 7]);
         }
-        e0 = fminf(fminf(e0, e1), fminf(e2, e3));
+        e0 = min3(e0, s[kKeys - 4], s[kKeys - 3]);
+        e1 = min3(e1, s[kKeys - 2], s[kKeys - 1]);
+        e0 = fminf(min3(e0, e1, e2), e3);
       }
       const float top = e0 * c;
       if (n == 0) {
@@ -432,25 +439,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // All scores -inf so far: 2^(-inf - 0) = 0, not NaN.
       const float ref = m == -INFINITY ? 0.f : m;
-      float l0 = 0.f, l1 = 0.f;
+      const float2 c2 = splat2(c), r2 = splat2(-ref);
+      float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float p[32];
 #pragma unroll
         for (int x = 0; x < 32; ++x) {
-          const float p0 = ex2_approx(fmaf(s[64 * h + 2 * x], c, -ref));
-          const float p1 = ex2_approx(fmaf(s[64 * h + 2 * x + 1], c, -ref));
-          l0 += p0;
-          l1 += p1;
-          p[x] = __uint_as_float(pack2<T>(p0, p1));
+          const float2 t = fma2(make_float2(s[64 * h + 2 * x], s[64 * h + 2 * x + 1]), c2, r2);
+          const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
+          sum = add2(sum, e);
+          p[x] = __uint_as_float(pack2<T>(e.x, e.y));
         }
         tmem_st_32x32b_x32(s_col + 32 * h, p);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(h == 0 ? &p_half[i] : &p_full[i]);
       }
-      l += l0 + l1;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i]);
+      l += sum.x + sum.y;
     }
     if (ok && mine > 0)
       ok = warp_wait_x(&pv_done[i], (mine - 1) & 1, err, kErrWaitAccFull, lane);

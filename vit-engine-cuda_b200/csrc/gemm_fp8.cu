@@ -61,6 +61,7 @@ struct Fp8GemmArgs {
   void* out;
   int64_t ldo;
   int gelu;
+  int vec_xs;         // rows of X's scales take four at a time
   int tma_out;        // the result goes out through tmap_out
   int tma_res;        // the residual comes in through tmap_res
   int vec;            // tile kernel: out, residual and bias take four columns at a time
@@ -110,48 +111,59 @@ __device__ __forceinline__ void drain_wait8(uint64_t* bar, uint32_t parity, int*
   }
 }
 
-// sum[i] += s * (32 * COLS32 accumulator columns from taddr): each load of 32
-// columns is in flight while the previous 32 are added.
-template <int COLS32>
-__device__ __forceinline__ void drain_block(uint32_t taddr, float s, float (&sum)[32 * COLS32]) {
-  uint32_t r[2][32];
-  tmem_ld_issue_x32(taddr, r[0]);
+// sum[i] += s * (column i of the accumulator at taddr), 16 columns at a time,
+// each load in flight while the previous 16 are added; `release` runs as soon as
+// the last has arrived. (Loads of 32 columns spilled and ran 3 % slower.)
+template <int COLS, typename Release>
+__device__ __forceinline__ void drain_block(uint32_t taddr, float s, float2 (&sum)[COLS / 2],
+                                            Release&& release) {
+  const float2 s2 = splat2(s);
+  uint32_t r[2][16];
+  tmem_ld_issue_x16(taddr, r[0]);
 #pragma unroll
-  for (int i = 0; i < COLS32; ++i) {
-    tmem_ld_wait_x32(r[i & 1]);
-    if (i + 1 < COLS32)
-      tmem_ld_issue_x32(taddr + static_cast<uint32_t>(32 * (i + 1)), r[(i + 1) & 1]);
+  for (int i = 0; i < COLS / 16; ++i) {
+    uint32_t(&t)[16] = r[i & 1];
+    tmem_ld_wait_x16(t);
+    if (i + 1 < COLS / 16)
+      tmem_ld_issue_x16(taddr + static_cast<uint32_t>(16 * (i + 1)), r[(i + 1) & 1]);
+    else
+      release();
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-      sum[32 * i + c] = fmaf(s, __uint_as_float(r[i & 1][c]), sum[32 * i + c]);
+    for (int c = 0; c < 8; ++c)
+      sum[8 * i + c] =
+          fma2(s2, make_float2(__uint_as_float(t[2 * c]), __uint_as_float(t[2 * c + 1])),
+               sum[8 * i + c]);
   }
 }
 
 // ---------------------------------------------------------------- CTA pair
 constexpr int kPairBN = 256;
-constexpr int kPairStages = 6;
+constexpr int kWgCols = kPairBN / 2;             // columns of a tile an epilogue warpgroup owns
 constexpr int kPairBRows = kPairBN / 2;
 constexpr int kPairStageBytes = kABytes + kPairBRows * kBK;
+// Five stages: six measured the same (323 against 321 us at 16384 x 4096 x
+// 4096) and leave L1 too small for the scales' lines.
+constexpr int kPairStages = 5;
 constexpr int kPairBufs = kTmemAll / kPairBN;
-// Per epilogue warp: one 32-row x 32-column slab of the result or residual.
-constexpr int kSlabBytes = 32 * 32 * 4;
+// Per epilogue warp: one slab of the result or residual.
+constexpr int kSlabBytes = 32 * 128;
 constexpr int kPairSmem = kPairStages * kPairStageBytes + 8 * kSlabBytes + 1024;
 static_assert(kPairSmem <= 227 * 1024, "shared memory");
 // 384 threads launched at 168 registers; the control warpgroup drops to 56 and
-// the epilogue warpgroups (128 sums and two loads of 32 a thread) rise to 224:
+// the epilogue warpgroups (128 sums and two loads of 16 a thread) rise to 224:
 // 128 * 56 + 256 * 224 = 384 * 168. build.py checks that ptxas allocated 168.
+// Four epilogue warpgroups of 64 columns (104 registers) measured 322-357 us
+// against 317-322 here.
 constexpr uint32_t kPairCtrlRegs = 56;
 constexpr uint32_t kPairEpiRegs = 224;
 static_assert(128 * kPairCtrlRegs + 256 * kPairEpiRegs == kThreads * 168, "register split");
 
-// Where the 16-byte chunk q of slab row r lies: the swizzle of the tensor map
-// that stores the slab (128-byte rows of fp32: 128B; 64-byte rows of 16-bit
-// types: 64B), free of bank conflicts for a lane writing its own row.
+// A slab is 32 rows of 128 bytes: the 16-byte chunk q of row r lies where the
+// 128-byte swizzle of the tensor map that stores it puts it, which also keeps a
+// lane writing its own row free of bank conflicts.
+__device__ __forceinline__ int slab_at(int r, int q) { return r * 128 + 16 * (q ^ (r & 7)); }
 template <typename T>
-__device__ __forceinline__ int slab_at(int r, int q) {
-  if constexpr (sizeof(T) == 4) return r * 128 + 16 * (q ^ (r & 7));
-  return r * 64 + 16 * (q ^ ((r >> 1) & 3));
-}
+constexpr int kSlabCols = 128 / sizeof(T);
 
 template <typename T>
 __device__ __forceinline__ void add_chunk(const uint8_t* p, float* v) {
@@ -169,57 +181,66 @@ __device__ __forceinline__ void put_chunk(uint8_t* p, const float* v) {
   *reinterpret_cast<uint4*>(p) = t;
 }
 
-// Epilogue of a warp's 32 x 32 slab (lane i = row m_base + i, columns n0..),
-// warp-collective. `slab` is the warp's buffer, `res_bar` its residual barrier.
+// Epilogue of a warp's slab (lane i = row m_base + i, columns n0..), warp-
+// collective. `slab` is the warp's buffer, `res_bar` its residual barrier.
 template <typename T>
 __device__ __forceinline__ void finish_slab(const Fp8GemmArgs& a, int64_t m_base, int lane, int n0,
-                                            float (&v)[32], uint8_t* slab,
+                                            float2* v, uint8_t* slab,
                                             const CUtensorMap* tmap_out,
                                             const CUtensorMap* tmap_res, uint64_t* res_bar,
                                             uint32_t& res_phase) {
+  constexpr int kCols = kSlabCols<T>;
   constexpr int kPer = 16 / sizeof(T);  // columns per 16-byte chunk
   const int64_t m = m_base + lane;
-  const bool full = n0 + 32 <= a.N;
-  if (a.tma_out || a.tma_res) {
-    if (lane == 0) bulk_wait_group_read<0>();  // the previous slab's store has read the buffer
-    __syncwarp();
-  }
   if (a.tma_res && lane == 0) {
-    mbar_arrive_expect_tx(res_bar, 32 * 32 * sizeof(T));
+    bulk_wait_group_read<0>();  // the previous slab's store has read the buffer
+    mbar_arrive_expect_tx(res_bar, kSlabBytes);
     tma_load_2d(slab, tmap_res, res_bar, n0, static_cast<int>(m_base));
   }
   if (a.bias != nullptr) {
-    if (full && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
+    if (n0 + kCols <= a.N && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) {
-        const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + n0 + j));
-        v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+      for (int j = 0; j < kCols / 4; ++j) {
+        const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + n0) + j);
+        v[2 * j] = add2(v[2 * j], make_float2(b.x, b.y));
+        v[2 * j + 1] = add2(v[2 * j + 1], make_float2(b.z, b.w));
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] += n0 + j < a.N ? __ldg(a.bias + n0 + j) : 0.f;
+      for (int j = 0; j < kCols / 2; ++j) {
+        v[j].x += n0 + 2 * j < a.N ? __ldg(a.bias + n0 + 2 * j) : 0.f;
+        v[j].y += n0 + 2 * j + 1 < a.N ? __ldg(a.bias + n0 + 2 * j + 1) : 0.f;
+      }
     }
   }
   if (a.gelu) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = gelu_erf(v[j]);
+    for (int j = 0; j < kCols / 2; ++j) v[j] = gelu_erf2(v[j]);
   }
   if (a.tma_res) {
     if (!mbar_wait(res_bar, res_phase, a.err, kErrWaitFull)) drain_wait8(res_bar, res_phase, a.err);
     res_phase ^= 1u;
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; j += kPer) add_chunk<T>(slab + slab_at<T>(lane, j / kPer), v + j);
+    for (int q = 0; q < 8; ++q)
+      add_chunk<T>(slab + slab_at(lane, q), reinterpret_cast<float*>(v + q * kPer / 2));
     __syncwarp();
   } else if (a.residual != nullptr && m < a.M) {
     const T* r = static_cast<const T*>(a.residual) + m * a.ldr + n0;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n0 + j < a.N) v[j] = to_f32(r[j]) + v[j];
+    for (int j = 0; j < kCols / 2; ++j) {
+      if (n0 + 2 * j < a.N) v[j].x = to_f32(r[2 * j]) + v[j].x;
+      if (n0 + 2 * j + 1 < a.N) v[j].y = to_f32(r[2 * j + 1]) + v[j].y;
+    }
   }
   if (a.tma_out) {
+    if (!a.tma_res) {
+      if (lane == 0) bulk_wait_group_read<0>();
+      __syncwarp();
+    }
 #pragma unroll
-    for (int j = 0; j < 32; j += kPer) put_chunk<T>(slab + slab_at<T>(lane, j / kPer), v + j);
+    for (int q = 0; q < 8; ++q)
+      put_chunk<T>(slab + slab_at(lane, q), reinterpret_cast<const float*>(v + q * kPer / 2));
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
@@ -229,9 +250,26 @@ __device__ __forceinline__ void finish_slab(const Fp8GemmArgs& a, int64_t m_base
   } else if (m < a.M) {
     T* o = static_cast<T*>(a.out) + m * a.ldo + n0;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n0 + j < a.N) o[j] = from_f32<T>(v[j]);
+    for (int j = 0; j < kCols / 2; ++j) {
+      if (n0 + 2 * j < a.N) o[2 * j] = from_f32<T>(v[j].x);
+      if (n0 + 2 * j + 1 < a.N) o[2 * j + 1] = from_f32<T>(v[j].y);
+    }
   }
+}
+
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  asm volatile("prefetch.global.L1 [%0];" ::"l"(p));
+}
+
+// A row's scales of K blocks kb .. kb + 3 (those past the last are not read).
+__device__ __forceinline__ float4 load_scales(const float* xs, int kb, int num_kb, int vec) {
+  if (vec && kb + 4 <= num_kb) return __ldg(reinterpret_cast<const float4*>(xs + kb));
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (kb < num_kb) v.x = __ldg(xs + kb);
+  if (kb + 1 < num_kb) v.y = __ldg(xs + kb + 1);
+  if (kb + 2 < num_kb) v.z = __ldg(xs + kb + 2);
+  if (kb + 3 < num_kb) v.w = __ldg(xs + kb + 3);
+  return v;
 }
 
 // Output tile `t`: row blocks run fastest inside bands of kBandN column tiles,
@@ -255,8 +293,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                          const __grid_constant__ CUtensorMap tmap_res, const Fp8GemmArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[kPairStages];
-  __shared__ __align__(8) uint64_t empty_bar[kPairStages];
-  __shared__ __align__(8) uint64_t acc_full_bar[kPairBufs];
+  // A K block's products are done: its stage is free and its accumulator full.
+  // One barrier serves producer and epilogue, so a block costs one commit. The
+  // epilogue cannot fall a turn of the ring behind: block s + kPairStages needs
+  // an accumulator that every warp has drained after block s.
+  __shared__ __align__(8) uint64_t done_bar[kPairStages];
   __shared__ __align__(8) uint64_t acc_empty_bar[kPairBufs];
   __shared__ __align__(8) uint64_t mma_done_bar;
   __shared__ __align__(8) uint64_t res_bar[8];
@@ -275,10 +316,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
       mbar_init(&full_bar[s], 1);
-      mbar_init(&empty_bar[s], 1);
+      mbar_init(&done_bar[s], 1);
     }
     for (int b = 0; b < kPairBufs; ++b) {
-      mbar_init(&acc_full_bar[b], 1);
       mbar_init(&acc_empty_bar[b], 16);  // every epilogue warp of both CTAs
     }
     mbar_init(&mma_done_bar, 1);
@@ -316,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int x_row = mb * 2 * kBM + static_cast<int>(rank) * kBM;
         const int w_row = nb * kPairBN + static_cast<int>(rank) * kPairBRows;
         for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, err, kErrWaitEmpty)) {
+          if (!mbar_wait(&done_bar[stage], phase ^ 1u, err, kErrWaitEmpty)) {
             ok = false;
             break;
           }
@@ -345,11 +385,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       uint32_t seq = 0;  // K blocks so far: accumulator seq % 2, its use seq / 2
       bool ok = true;
-      auto commit = [&](uint64_t* bar) {
-        const uint32_t addr = smem_addr(bar);
-        umma_commit_pair(addr);
-        umma_commit_pair(mapa_shared(addr, 1));
-      };
       for (int t = unit; t < a.num_tiles && ok; t += num_units) {
         for (int kb = 0; kb < num_kb; ++kb, ++seq) {
           const int buf = static_cast<int>(seq % kPairBufs);
@@ -367,8 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)  // 32 columns = 32 bytes = +2 in the address field
             umma_f8_pair(d, dx + 2 * kk, dw + 2 * kk, kIdesc, kk ? 1u : 0u);
-          commit(&empty_bar[stage]);
-          commit(&acc_full_bar[buf]);
+          umma_commit_both(&done_bar[stage]);
           if (++stage == kPairStages) stage = 0, phase ^= 1u;
         }
       }
@@ -384,55 +418,70 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                               static_cast<uint32_t>(wg * 128);
+                               static_cast<uint32_t>(wg * kWgCols);
     uint8_t* slab = ring + kPairStages * kPairStageBytes + (warp - 4) * kSlabBytes;
     uint32_t res_phase = 0;
     uint32_t seq = 0;
+    int stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int t = unit; t < a.num_tiles && ok; t += num_units) {
       int mb, nb;
       tile_at(t, m_tiles, a.num_n_tiles, mb, nb);
       const int64_t m_base = static_cast<int64_t>(mb) * 2 * kBM + rank * kBM + quarter * 32;
-      const int n_base = nb * kPairBN + wg * 128;
+      const int n_base = nb * kPairBN + wg * kWgCols;
       // Tiles at the edges: warps whose rows or columns lie outside read nothing.
       const bool live = m_base < a.M && n_base < a.N;
       const float* xs = a.xs + (m_base + lane < a.M ? m_base + lane : a.M - 1) * a.ldxs;
       const float* ws = a.ws + static_cast<int64_t>(live ? n_base / kFp8Block : 0) * a.ldws;
-      float sum[128];
+      float2 sum[kWgCols / 2];
 #pragma unroll
-      for (int c = 0; c < 128; ++c) sum[c] = 0.f;
-      float s = __ldg(xs) * __ldg(ws);
+      for (int c = 0; c < kWgCols / 2; ++c) sum[c] = make_float2(0.f, 0.f);
+      if (a.bias != nullptr && n_base + 4 * lane < a.N) prefetch_l1(a.bias + n_base + 4 * lane);
+      float4 sx = load_scales(xs, 0, num_kb, a.vec_xs), sx_next = sx;
+      float sw = __ldg(ws);
       for (int kb = 0; kb < num_kb; ++kb, ++seq) {
         const int buf = static_cast<int>(seq % kPairBufs);
-        const int next = kb + 1 < num_kb ? kb + 1 : kb;
-        const float xs_next = __ldg(xs + next), ws_next = __ldg(ws + next);
-        if (!warp_wait8(&acc_full_bar[buf], (seq / kPairBufs) & 1u, err, kErrWaitAccFull, lane)) {
+        const int u = kb & 3;
+        if (u == 0) {
+          sx = sx_next;
+          sx_next = load_scales(xs, kb + 4, num_kb, a.vec_xs);
+        }
+        const float s = sw * (u & 2 ? (u & 1 ? sx.w : sx.z) : (u & 1 ? sx.y : sx.x));
+        sw = __ldg(ws + (kb + 1 < num_kb ? kb + 1 : kb));
+        if (!mbar_wait(&done_bar[stage], phase, err, kErrWaitAccFull)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (live) drain_block<4>(lane_base + static_cast<uint32_t>(buf * kPairBN), s, sum);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if (leader)
-            mbar_arrive(&acc_empty_bar[buf]);
-          else
-            mbar_arrive_cluster(mapa_shared(smem_addr(&acc_empty_bar[buf]), 0));
-        }
-        s = xs_next * ws_next;
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (leader)
+              mbar_arrive(&acc_empty_bar[buf]);
+            else
+              mbar_arrive_remote(mapa_shared(smem_addr(&acc_empty_bar[buf]), 0));
+          }
+        };
+        if (live)
+          drain_block<kWgCols>(lane_base + static_cast<uint32_t>(buf * kPairBN), s, sum, release);
+        else
+          release();
+        if (++stage == kPairStages) stage = 0, phase ^= 1u;
       }
       if (!ok) break;
       if (live) {
-        // One copy of the slab code: the sums move down by 32 registers after each.
+        // One copy of the slab code: the sums move down by a slab after each.
+        constexpr int kCols = kSlabCols<T>;
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int n0 = n_base + 32 * i;
+        for (int n0 = n_base; n0 < n_base + kWgCols; n0 += kCols) {
           if (n0 < a.N)
-            finish_slab<T>(a, m_base, lane, n0, *reinterpret_cast<float(*)[32]>(&sum[0]), slab,
-                           &tmap_out, &tmap_res, &res_bar[warp - 4], res_phase);
+            finish_slab<T>(a, m_base, lane, n0, sum, slab, &tmap_out, &tmap_res,
+                           &res_bar[warp - 4], res_phase);
 #pragma unroll
-          for (int c = 0; c < 96; ++c) sum[c] = sum[c + 32];
+          for (int c = 0; c < (kWgCols - kCols) / 2; ++c) sum[c] = sum[c + kCols / 2];
         }
       }
     }
@@ -581,9 +630,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                                static_cast<uint32_t>(wg * Cfg::kWgCols);
     const float* xs = a.xs + (m < a.M ? m : a.M - 1) * a.ldxs;
     const float* ws = a.ws + static_cast<int64_t>(live ? n_base / kFp8Block : 0) * a.ldws;
-    float sum[Cfg::kWgCols];
+    float2 sum[Cfg::kWgCols / 2];
 #pragma unroll
-    for (int c = 0; c < Cfg::kWgCols; ++c) sum[c] = 0.f;
+    for (int c = 0; c < Cfg::kWgCols / 2; ++c) sum[c] = make_float2(0.f, 0.f);
     float s = __ldg(xs + kb0) * __ldg(ws + kb0);
     bool ok = true;
     for (int kb = kb0; kb < kb1; ++kb) {
@@ -596,11 +645,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc_fence_after();
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty_bar[buf]);
+      };
       if (live)
-        drain_block<Cfg::kWgCols / 32>(lane_base + static_cast<uint32_t>(buf * BN), s, sum);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty_bar[buf]);
+        drain_block<Cfg::kWgCols>(lane_base + static_cast<uint32_t>(buf * BN), s, sum, release);
+      else
+        release();
       s = xs_next * ws_next;
     }
     // The last block's accumulator is complete, so every product has read the
@@ -611,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int c = 0; c < Cfg::kWgCols; c += 4)
         *reinterpret_cast<float4*>(part + row * Cfg::kPitch + wg * Cfg::kWgCols + c) =
-            make_float4(sum[c], sum[c + 1], sum[c + 2], sum[c + 3]);
+            make_float4(sum[c / 2].x, sum[c / 2].y, sum[c / 2 + 1].x, sum[c / 2 + 1].y);
     }
   }
   __syncwarp();
@@ -712,8 +765,8 @@ int launch_pair(const Fp8GemmProblem& p, Fp8GemmArgs& a, cudaStream_t s) {
   auto slab_map = [&](CUtensorMap* map, const void* base, int64_t ld) {
     const uint64_t dims[2] = {static_cast<uint64_t>(p.N), static_cast<uint64_t>(p.M)};
     const uint64_t strides[1] = {static_cast<uint64_t>(ld) * sizeof(T)};
-    const uint32_t box[2] = {32, 32};
-    return encode_tmap_typed(map, 2, base, dims, strides, box, sizeof(T) == 4, sizeof(T) == 2);
+    const uint32_t box[2] = {kSlabCols<T>, 32};
+    return encode_tmap_typed(map, 2, base, dims, strides, box, 1, sizeof(T) == 2);
   };
   to = tr = tx;
   a.tma_out = aligned(p.out, p.ldo * sizeof(T), 16);
@@ -782,6 +835,7 @@ int gemm_fp8_launch(const Fp8GemmProblem& p, cudaStream_t s) {
   a.out = p.out;
   a.ldo = p.ldo;
   a.gelu = p.gelu;
+  a.vec_xs = aligned(p.xs, p.ldxs * 4, 16);
   a.err = device_error_word();
   const int sms = device_num_sms();
   const int64_t pair_tiles = (p.M + 2 * kBM - 1) / (2 * kBM) * ((p.N + kPairBN - 1) / kPairBN);
