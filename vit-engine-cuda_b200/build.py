@@ -1,4 +1,6 @@
-"""Builds libvitb200.so (the sm_100a kernels + C ABI) in-tree with nvcc.
+"""Builds libvitb200.so (the sm_100a kernels + C ABI) in-tree with nvcc, and
+_serving.so (csrc/bindings.cpp: the serving operators' Python entry points,
+compiled against the installed PyTorch) with g++.
 
     python vit-engine-cuda_b200/build.py [--force] [--jobs N]
 
@@ -10,11 +12,13 @@ GPU (the kernels themselves need an sm_100a device).
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -24,6 +28,8 @@ INCLUDE = os.path.join(REPO, "include")
 OUT_DIR = os.path.join(HERE, "vit_cuda")
 LIB = os.path.join(OUT_DIR, "libvitb200.so")
 OBJ_DIR = os.path.join(HERE, "_build")
+BINDINGS = os.path.join(CSRC, "bindings.cpp")
+BINDINGS_LIB = os.path.join(OUT_DIR, "_serving.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -50,11 +56,36 @@ def headers() -> list[str]:
     return hs
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def newer_than(lib: str, inputs: list[str]) -> bool:
+    if not os.path.exists(lib):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(f) <= t for f in sources() + headers() + [__file__])
+    t = os.path.getmtime(lib)
+    return all(os.path.getmtime(f) <= t for f in inputs)
+
+
+def up_to_date() -> bool:
+    return newer_than(LIB, sources() + headers() + [__file__])
+
+
+def build_bindings(force: bool = False) -> str:
+    header = os.path.join(INCLUDE, "vitb200.h")
+    if not force and newer_than(BINDINGS_LIB, [BINDINGS, header, __file__]):
+        return BINDINGS_LIB
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    includes = [os.path.join(torch_dir, "include"),
+                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+                os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
+    tmp = BINDINGS_LIB + ".tmp"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared",
+           "-fvisibility=hidden", *(f"-I{d}" for d in includes), BINDINGS, "-o", tmp,
+           f"-L{os.path.join(torch_dir, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch_cuda", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDINGS}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDINGS_LIB)
+    return BINDINGS_LIB
 
 
 def compile_one(src: str) -> tuple[str, str]:
@@ -100,6 +131,14 @@ def check_register_split(ptxas_log: str) -> None:
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> str:
+    with ThreadPoolExecutor(max_workers=1) as ex:
+        bindings = ex.submit(build_bindings, force)
+        lib = build_library(force, jobs, verbose)
+        bindings.result()
+    return lib
+
+
+def build_library(force: bool = False, jobs: int | None = None, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB
     os.makedirs(OBJ_DIR, exist_ok=True)

@@ -260,6 +260,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
   }
 }
 
+// One lane of a converged warp, chosen by the hardware: the compiler then knows
+// that a single thread runs what follows and keeps descriptors and addresses in
+// uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- TMA ---------------------------------------------------------------
 // 3-D tiled bulk-tensor load global -> shared (this CTA only),
 // completion signalled on `bar` via complete_tx.

@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     setmaxnreg_dec<kCtrlRegs>();
-    if (warp == 0 && lane == 0 && nk > 0) {
+    if (warp == 0 && nk > 0 && elect_one()) {
       // -------------------------------------------------------------- TMA
       mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(it.tiles * C::kHalves * a.group *
                                                            a.tile_t * kHalf * 2));
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int s = 0; s < C::kVSlots; ++s)
         if (v_issued > s)
           drain_wait_x(&v_full[s], ((v_issued - 1 - s) / C::kVSlots) & 1, err);
-    } else if (warp == 1 && lane == 0 && nk > 0) {
+    } else if (warp == 1 && nk > 0 && elect_one()) {
       // -------------------------------------------------------------- MMA
       constexpr uint32_t kIdescS = idesc<T>(kKeys, false);
       constexpr uint32_t kIdescPV = idesc<T>(D, true);
@@ -316,12 +316,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The first half of the keys while the exponentials of the second run.
         if (!mbar_wait(&p_half[i], n & 1, err, kErrWaitAccFull)) return false;
         tc_fence_after();
-        for (int kk = 0; kk < min(4, steps); ++kk)  // 16 keys: 2048 bytes of V, 8 columns of P
-          umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
-        if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
-        tc_fence_after();
-        for (int kk = 4; kk < steps; ++kk)
-          umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+        // 16 keys a product: 2048 bytes of V, 8 columns of P. The full tile is
+        // unrolled: one thread issues every product, and a loop's own instructions
+        // between products of 64 cycles show.
+        if (steps == 8) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, kk ? 1u : (n ? 1u : 0u));
+          if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk)
+            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+        } else {
+          for (int kk = 0; kk < min(4, steps); ++kk)
+            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
+          if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+          tc_fence_after();
+          for (int kk = 4; kk < steps; ++kk)
+            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+        }
         umma_commit(&pv_done[i]);
         if (!shared_keys || i == 1) umma_commit(&v_empty[s]);
         return true;

@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     setmaxnreg_dec<kPairCtrlRegs>();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       // ------------------------------------------------------------ TMA
       int stage = 0;
       uint32_t phase = 0;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             drain_wait8(&full_bar[s], static_cast<uint32_t>((fills - 1) & 1), err);
           }
       }
-    } else if (warp == 1 && lane == 0 && leader) {
+    } else if (warp == 1 && leader && elect_one()) {
       // ------------------------------------------------------------ MMA
       constexpr uint32_t kIdesc = make_idesc_f8(2 * kBM, kPairBN);
       int stage = 0;
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t m_tile = static_cast<int64_t>(mb) * kBM;
   float* part = reinterpret_cast<float*>(ring);  // [128][kPitch] once the ring is idle
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0 && elect_one()) {
     // -------------------------------------------------------------- TMA
     int stage = 0;
     uint32_t phase = 0;
@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int fills = (issued - s + Cfg::kStages - 1) / Cfg::kStages;
         drain_wait8(&full_bar[s], static_cast<uint32_t>((fills - 1) & 1), err);
       }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1 && elect_one()) {
     // -------------------------------------------------------------- MMA
     // With a_rows < 128 the rows of the X tile past the box hold whatever was
     // there: they only reach output rows that do not exist.

@@ -117,8 +117,7 @@ def _(X, W, B):
 
 # ---------------------------------------------------------------- serving ops
 # vit_cuda.<op> calls these only while torch.compile traces; an eager call goes
-# straight to vit_cuda.serving, without the dispatcher's tens of microseconds,
-# which a single token's step would feel.
+# straight to vit_cuda.serving, without the dispatcher's tens of microseconds.
 def _fake_codes(X):
     K = X.shape[-1]
     ld = (K + 15) // 16 * 16
