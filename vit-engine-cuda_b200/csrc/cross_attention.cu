@@ -33,8 +33,8 @@
 #include <limits>
 #include <type_traits>
 
+#include "cross_attention.cuh"
 #include "engine.h"
-#include "fp8.cuh"
 
 namespace vitb200 {
 
@@ -51,7 +51,6 @@ static_assert(128 * kCtrlRegs + 256 * kSoftRegs == kThreads * 168, "register spl
 constexpr int kHalf = 64;                        // columns of one 128-byte swizzle span
 constexpr int kHalfBytes = kRows * kHalf * 2;    // 128 rows x 64 columns
 constexpr float kRescale = 8.f;                  // log2 of the largest P
-constexpr int kMaxSplit = 8;                     // portable cluster size
 
 template <int D>
 struct Cfg {
@@ -114,38 +113,6 @@ __device__ __forceinline__ void drain_wait_x(uint64_t* bar, uint32_t parity, int
       return;
     }
   }
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Floats of a partial result, in this CTA's shared memory or a peer's.
-__device__ __forceinline__ float ld_partial(uint32_t addr, bool remote) {
-  float v;
-  if (remote)
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_partial4(uint32_t addr, bool remote) {
-  if (remote) return ld_shared_cluster_f4(addr);
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
 }
 
 // A work item: a key head of an image and one or two of its row tiles.
@@ -605,7 +572,7 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   a.lens = p.lens;
   a.o = static_cast<uint16_t*>(p.o);
   a.o_row = static_cast<int64_t>(p.heads) * D;
-  a.c = p.scale * 1.44269504088896340736f;  // log2(e)
+  a.c = p.scale * kLog2e;
   // Masked scores are infinite, and infinity times zero is NaN: the smallest
   // float instead moves no score by more than 5e-7.
   if (a.c == 0.f) a.c = std::numeric_limits<float>::denorm_min();
@@ -619,10 +586,10 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   a.tile_t = std::min(kRows / a.group, p.Tq);
   a.nq = (p.Tq + a.tile_t - 1) / a.tile_t;
   const int64_t items = static_cast<int64_t>(p.B) * a.kv_heads * ((a.nq + 1) / 2);
-  if (items > INT32_MAX / kMaxSplit) return VITB200_E_UNSUPPORTED;
+  if (items > INT32_MAX / kCrossMaxSplit) return VITB200_E_UNSUPPORTED;
   const int key_tiles = std::max(1, (p.Tk + kKeys - 1) / kKeys);
   a.nsplit = static_cast<int>(std::max<int64_t>(
-      1, std::min<int64_t>({device_num_sms() / items, key_tiles, kMaxSplit})));
+      1, std::min<int64_t>({device_num_sms() / items, key_tiles, kCrossMaxSplit})));
 
   CUtensorMap tq, tk, tv;
   const uint64_t es = 2;
@@ -673,10 +640,12 @@ int cross_attention_prepare_device() {
       });
       if (st) return st;
     }
-  return 0;
+  return cross_attention_token_prepare_device();
 }
 
 int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
+  if (static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows)
+    return cross_attention_token_launch(p, s);
   return with_head(p.type, p.D, [&](auto tag, auto d) {
     return launch_tiles<decltype(tag), d.value>(p, s);
   });
