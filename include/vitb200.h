@@ -339,12 +339,17 @@ int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64
  * each image (clamped to 0..Tk), or NULL for Tk everywhere; keys past it are not
  * read into the result, whatever they hold. An image without keys gets zeros.
  * Scores, exponentials' sums and outputs are fp32, probabilities are rounded to
- * `type` for the product with V, o is rounded once. No workspace. No counterpart
- * in the reference (its attention has equal lengths, one type, 12 heads of 64). */
+ * `type` for the product with V, o is rounded once. The workspace (16-byte
+ * aligned; often 0 bytes, then NULL) holds parts of key heads that several CTAs
+ * share; calls whose GPU work can overlap need one each. No counterpart in the
+ * reference (its attention has equal lengths, one type, 12 heads of 64). */
+size_t vitb200_cross_attention_workspace_bytes(int B, int Tq, int Tk, int heads, int kv_heads,
+                                               int head_dim);
 int vitb200_cross_attention(const void* q, const void* k, const void* v, void* o, int type, int B,
                             int Tq, int Tk, int heads, int kv_heads, int head_dim, int64_t q_row,
                             int64_t q_batch, int64_t k_row, int64_t k_batch, int64_t v_row,
-                            int64_t v_batch, const int* kv_lens, float scale, void* stream);
+                            int64_t v_batch, const int* kv_lens, float scale, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 /* ---- whole-model forward (reference: vit_cuda/model.py:93-126) --------- */
 

@@ -101,6 +101,28 @@ def test_keys_past_the_length_are_never_seen(cuda, tq, d, bad):
     assert bool((o[0] == 0).all()) and bool((o[13] == 0).all())
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tq,heads,kv_heads", [(1, 8, 2), (1, 1, 1), (3, 4, 4), (1, 16, 1), (20, 4, 2)])
+@pytest.mark.parametrize("lens", [[0, 9000, 3, 4097, 17], [5, 0, 0, 0, 0], [0, 0, 0, 0, 0],
+                                  [9000, 9000, 8999, 1, 9000], [0, 0, 16, 33, 2000]])
+def test_long_ragged_lengths(cuda, d, tq, heads, kv_heads, lens):
+    """Work that is cut evenly whatever the lengths: key heads shared by several
+    CTAs, CTAs with several key heads, fewer steps than CTAs, empty images first,
+    last and between."""
+    lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q, k, v = operands(5, tq, 9000, heads, kv_heads, d, torch.bfloat16, seed=50)
+    o = vit_cuda.cross_attention(q, k, v, d ** -0.5, heads, kv_heads, lens)
+    check(o, q, k, v, d ** -0.5, heads, kv_heads, lens)
+    assert bool((o[lens == 0] == 0).all())
+
+
+def test_many_images(cuda):
+    """More images than a warp scans at once."""
+    lens = torch.arange(100, dtype=torch.int32, device="cuda") * 97 % 3001
+    q, k, v = operands(100, 1, 3000, 4, 1, 64, torch.float16, seed=51)
+    check(vit_cuda.cross_attention(q, k, v, 0.125, 4, 1, lens), q, k, v, 0.125, 4, 1, lens)
+
+
 @pytest.mark.parametrize("tq", [1, 40, 300])
 def test_bad_values_within_the_length(cuda, tq):
     """A NaN key or query makes its rows NaN, a NaN value its column; other

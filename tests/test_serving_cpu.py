@@ -58,7 +58,7 @@ def test_gemm_status():
 def cross(q=P, k=P, v=P, o=P, type=1, B=2, Tq=3, Tk=5, heads=4, kv_heads=2, D=64, qs=(256, 768),
           ks=(128, 640), vs=(128, 640), lens=None):
     return lib.vitb200_cross_attention(q, k, v, o, type, B, Tq, Tk, heads, kv_heads, D, *qs, *ks,
-                                       *vs, lens, 0.125, None)
+                                       *vs, lens, 0.125, None, 0, None)
 
 
 def test_cross_attention_status():

@@ -5,7 +5,7 @@
 // against 3-6 us on the GPU for a single token's step; these functions take
 // their arguments by position from the interpreter's own vector and spend 4-5
 // us, most of it the launch itself. The package opens libvitb200.so (ctypes) and
-// hands the four entry points' addresses to `bind`, so this module links only
+// hands the entry points' addresses to `bind`, so this module links only
 // PyTorch.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/Dtype.h>
@@ -27,6 +27,7 @@ struct Library {
   decltype(&vitb200_layernorm_fp8) layernorm = nullptr;
   decltype(&vitb200_gemm_fp8) gemm = nullptr;
   decltype(&vitb200_cross_attention) attention = nullptr;
+  decltype(&vitb200_cross_attention_workspace_bytes) attention_workspace = nullptr;
   PyObject* error = nullptr;  // raise_status(what, status)
 } g_lib;
 
@@ -311,22 +312,28 @@ PyObject* cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const Operand q = operand(Q), k = operand(K), v = operand(V);
   at::Tensor O = empty(Q.sizes(), type, device);
+  at::Tensor workspace;
+  const size_t bytes = g_lib.attention_workspace(
+      static_cast<int>(B), static_cast<int>(Tq), static_cast<int>(Tk), static_cast<int>(heads),
+      static_cast<int>(kv_heads), static_cast<int>(D));
+  if (bytes > 0) workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, device);
   const int st = g_lib.attention(
       q.t.data_ptr(), k.t.data_ptr(), v.t.data_ptr(), O.data_ptr(), type_code(type, "Q"),
       static_cast<int>(B), static_cast<int>(Tq), static_cast<int>(Tk), static_cast<int>(heads),
       static_cast<int>(kv_heads), static_cast<int>(D), q.row, q.batch, k.row, k.batch, v.row,
       v.batch, lens.defined() ? static_cast<const int*>(lens.data_ptr()) : nullptr, scale,
-      stream_of(device));
+      bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(device));
   return passed(st, op) ? THPVariable_Wrap(std::move(O)) : nullptr;
   END_HANDLE_TH_ERRORS
 }
 
-// (quantize, layernorm, gemm, attention: addresses in libvitb200.so; raise_status)
+// (quantize, layernorm, gemm, attention, attention_workspace: addresses in
+// libvitb200.so; raise_status)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK(n == 5, "bind takes four addresses and a function");
-  void* at[4];
-  for (int i = 0; i < 4; ++i) {
+  TORCH_CHECK(n == 6, "bind takes five addresses and a function");
+  void* at[5];
+  for (int i = 0; i < 5; ++i) {
     at[i] = PyLong_AsVoidPtr(args[i]);
     if (!at[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "bind: null address");
@@ -336,9 +343,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g_lib.quantize = reinterpret_cast<decltype(g_lib.quantize)>(at[0]);
   g_lib.layernorm = reinterpret_cast<decltype(g_lib.layernorm)>(at[1]);
   g_lib.attention = reinterpret_cast<decltype(g_lib.attention)>(at[3]);
-  Py_INCREF(args[4]);
+  g_lib.attention_workspace = reinterpret_cast<decltype(g_lib.attention_workspace)>(at[4]);
+  Py_INCREF(args[5]);
   Py_XDECREF(g_lib.error);
-  g_lib.error = args[4];
+  g_lib.error = args[5];
   g_lib.gemm = reinterpret_cast<decltype(g_lib.gemm)>(at[2]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

@@ -588,8 +588,12 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   const int64_t items = static_cast<int64_t>(p.B) * a.kv_heads * ((a.nq + 1) / 2);
   if (items > INT32_MAX / kCrossMaxSplit) return VITB200_E_UNSUPPORTED;
   const int key_tiles = std::max(1, (p.Tk + kKeys - 1) / kKeys);
+  // The largest cluster of which `items` fit the GPU at once.
   a.nsplit = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>({device_num_sms() / items, key_tiles, kCrossMaxSplit})));
+  while (a.nsplit > 1 &&
+         cluster_slots(cross_attention_kernel<T, D>, C::kSmem, kThreads, a.nsplit) < items)
+    --a.nsplit;
 
   CUtensorMap tq, tk, tv;
   const uint64_t es = 2;
@@ -643,9 +647,18 @@ int cross_attention_prepare_device() {
   return cross_attention_token_prepare_device();
 }
 
+namespace {
+bool token_form(const CrossProblem& p) {
+  return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows;
+}
+}  // namespace
+
+size_t cross_attention_workspace(const CrossProblem& p) {
+  return token_form(p) ? cross_attention_token_workspace(p) : 0;
+}
+
 int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
-  if (static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows)
-    return cross_attention_token_launch(p, s);
+  if (token_form(p)) return cross_attention_token_launch(p, s);
   return with_head(p.type, p.D, [&](auto tag, auto d) {
     return launch_tiles<decltype(tag), d.value>(p, s);
   });
@@ -655,24 +668,57 @@ int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
 
 using namespace vitb200;
 
+namespace {
+
+// Sizes of the operator; a status where they make none.
+int cross_sizes(int type, int B, int Tq, int Tk, int heads, int kv_heads, int head_dim,
+                CrossProblem* p) {
+  if (type != VITB200_F16 && type != VITB200_BF16) return VITB200_E_INVALID_ARG;
+  if (B < 0 || Tq < 0 || Tk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
+    return VITB200_E_INVALID_ARG;
+  if (head_dim != 64 && head_dim != 128) return VITB200_E_UNSUPPORTED;
+  if (Tq > INT32_MAX - 256 || Tk > INT32_MAX - 256 || heads > 65535) return VITB200_E_UNSUPPORTED;
+  p->type = type;
+  p->B = B;
+  p->Tq = Tq;
+  p->Tk = Tk;
+  p->heads = heads;
+  p->kv_heads = kv_heads;
+  p->D = head_dim;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" size_t vitb200_cross_attention_workspace_bytes(int B, int Tq, int Tk, int heads,
+                                                          int kv_heads, int head_dim) {
+  try {
+    CrossProblem p = {};
+    if (cross_sizes(VITB200_BF16, B, Tq, Tk, heads, kv_heads, head_dim, &p) || B == 0 || Tq == 0 ||
+        Tk == 0)
+      return 0;
+    return cross_attention_workspace(p);
+  } catch (...) {
+    return 0;
+  }
+}
+
 extern "C" int vitb200_cross_attention(const void* q, const void* k, const void* v, void* o,
                                        int type, int B, int Tq, int Tk, int heads, int kv_heads,
                                        int head_dim, int64_t q_row, int64_t q_batch, int64_t k_row,
                                        int64_t k_batch, int64_t v_row, int64_t v_batch,
-                                       const int* kv_lens, float scale, void* stream) {
+                                       const int* kv_lens, float scale, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
   try {
-    if (type != VITB200_F16 && type != VITB200_BF16) return VITB200_E_INVALID_ARG;
-    if (B < 0 || Tq < 0 || Tk < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0)
-      return VITB200_E_INVALID_ARG;
-    if (head_dim != 64 && head_dim != 128) return VITB200_E_UNSUPPORTED;
-    if (Tq > INT32_MAX - 256 || Tk > INT32_MAX - 256 || heads > 65535) return VITB200_E_UNSUPPORTED;
+    CrossProblem p = {};
+    if (int st = cross_sizes(type, B, Tq, Tk, heads, kv_heads, head_dim, &p)) return st;
     const int64_t wq = static_cast<int64_t>(heads) * head_dim;
     const int64_t wk = static_cast<int64_t>(kv_heads) * head_dim;
     if (q_row < wq || k_row < wk || v_row < wk || q_batch < 0 || k_batch < 0 || v_batch < 0)
       return VITB200_E_INVALID_ARG;
     if (B == 0 || Tq == 0) return 0;
     if (!q || !o || (Tk > 0 && (!k || !v))) return VITB200_E_INVALID_ARG;
-    for (const void* t : {q, k, v, static_cast<const void*>(o)})
+    for (const void* t : {q, k, v, static_cast<const void*>(o), static_cast<const void*>(workspace)})
       if (reinterpret_cast<uintptr_t>(t) % 16 != 0) return VITB200_E_ALIGNMENT;
     for (int64_t st : {q_row, q_batch, k_row, k_batch, v_row, v_batch})
       if (st % 8 != 0) return VITB200_E_ALIGNMENT;
@@ -681,19 +727,13 @@ extern "C" int vitb200_cross_attention(const void* q, const void* k, const void*
     if (Tk == 0)
       return cuda_status(cudaMemsetAsync(o, 0, static_cast<size_t>(B) * Tq * wq * 2,
                                          static_cast<cudaStream_t>(stream)));
-    CrossProblem p = {};
+    const size_t need = cross_attention_workspace(p);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return VITB200_E_WORKSPACE;
     p.q = q;
     p.k = k;
     p.v = v;
     p.o = o;
     p.lens = kv_lens;
-    p.type = type;
-    p.B = B;
-    p.Tq = Tq;
-    p.Tk = Tk;
-    p.heads = heads;
-    p.kv_heads = kv_heads;
-    p.D = head_dim;
     p.q_row = q_row;
     p.q_batch = q_batch;
     p.k_row = k_row;
@@ -701,6 +741,7 @@ extern "C" int vitb200_cross_attention(const void* q, const void* k, const void*
     p.v_row = v_row;
     p.v_batch = v_batch;
     p.scale = scale;
+    p.workspace = workspace;
     return cross_attention_launch(p, static_cast<cudaStream_t>(stream));
   } catch (...) {
     return VITB200_E_INVALID_ARG;

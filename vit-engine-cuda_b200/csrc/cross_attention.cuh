@@ -20,15 +20,17 @@ struct CrossTokenArgs {
   const uint16_t* k;
   const uint16_t* v;
   uint16_t* o;
+  float* parts;     // workspace of the streaming form
   const int* lens;  // [B] or null
-  int Tq, Tk, kv_heads;
+  int B, Tq, Tk, kv_heads;
   int group;   // query heads per key head
   int rows;    // group * Tq <= 16
-  int nsplit;  // CTAs per key head
   float c;     // scale * log2(e)
   int64_t q_row, q_batch, k_row, k_batch, v_row, v_batch, o_row;
 };
 int cross_attention_token_prepare_device();
+// Bytes of workspace its launch needs (0 where a CTA per key head does).
+size_t cross_attention_token_workspace(const CrossProblem& p);
 int cross_attention_token_launch(const CrossProblem& p, cudaStream_t s);
 
 template <typename T>
@@ -63,13 +65,19 @@ __device__ __forceinline__ float4 ld_partial4(uint32_t addr, bool remote) {
   return v;
 }
 
-// Sixteen bytes that are read once: past L1.
-__device__ __forceinline__ uint4 ld_stream(const uint16_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// Sixteen bytes from global to shared memory, past L1; zeros where `inside` is
+// false (the address is not read then).
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool inside) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(inside ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 }  // namespace vitb200

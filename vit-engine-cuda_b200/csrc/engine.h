@@ -6,6 +6,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <map>
+#include <mutex>
+#include <tuple>
 #include <utility>
 
 namespace vitb200 {
@@ -216,7 +219,10 @@ struct CrossProblem {
   int B, Tq, Tk, heads, kv_heads, D;
   int64_t q_row, q_batch, k_row, k_batch, v_row, v_batch;
   float scale;
+  void* workspace;
 };
+// Bytes of workspace that the problem's launch needs (16-byte aligned; may be 0).
+size_t cross_attention_workspace(const CrossProblem& p);
 int cross_attention_launch(const CrossProblem& p, cudaStream_t s);
 // Raises shared-memory limits of its kernels on the current device.
 int cross_attention_prepare_device();
@@ -240,6 +246,41 @@ int xsplit_stats_launch(const float* x, int64_t ldx, int64_t rows, uint16_t* h16
 // Whether epilogues write their results through TMA tensor stores where they
 // can; on unless the environment sets VITB200_TMA_STORE=0.
 bool tma_store_enabled();
+
+// Clusters of `d` CTAs of this kernel that fit on the current device at once
+// (cached per kernel, device and d; 0 when the query fails).
+template <typename Kernel>
+int cluster_slots(Kernel kernel, int smem, int threads, int d) {
+  static std::mutex mu;
+  static std::map<std::tuple<Kernel, int, int, int>, int> cache;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  std::lock_guard<std::mutex> lock(mu);
+  auto [it, added] = cache.try_emplace({kernel, smem, dev, d}, 0);
+  if (added) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(d);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(d * (device_num_sms() / d)));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 0;
+    }
+    it->second = n;
+  }
+  return it->second;
+}
 
 // Launches `kernel` on `s` with the library's launch attributes: programmatic
 // stream serialization (when enabled) and, for cluster_x > 1, a cluster of

@@ -125,7 +125,9 @@ _SIGNATURES = {
                                  c_int64, _P, c_int64, c_int, c_int64, c_int, c_int, c_int, _P]),
     "vitb200_cross_attention": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int,
                                         c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
-                                        c_int64, _P, c_float, _P]),
+                                        c_int64, _P, c_float, _P, c_size_t, _P]),
+    "vitb200_cross_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int,
+                                                            c_int]),
     "vitb200_vit_workspace_bytes": (c_size_t, [POINTER(VitParams), c_int]),
     "vitb200_vit_forward": (c_int, [POINTER(VitParams), _P, _P, c_int, _P, c_size_t, _P]),
     "vitb200_vit_forward_features": (c_int, [POINTER(VitParams), _P, _P, c_int, _P, c_size_t,

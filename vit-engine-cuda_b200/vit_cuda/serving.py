@@ -5,8 +5,8 @@ block of 128 (``gemm_fp8``) and attention to an encoder's states of another leng
 
 They keep the manner of ``vit_cuda._C``: CUDA tensors on the current device
 (RuntimeError otherwise), fresh outputs from PyTorch's caching allocator, work
-launched asynchronously on the current stream, no workspace, capturable in a
-CUDA graph. They are forward only, like every op of this package.
+launched asynchronously on the current stream, scratch space from the caching
+allocator too, so that they can be captured in a CUDA graph. They are forward only, like every op of this package.
 
 The checks and the call into libvitb200.so are compiled (csrc/bindings.cpp, built
 as ``vit_cuda._serving``): in a single token's step the host's time per call is
@@ -46,7 +46,8 @@ def _load():
                                   "PyTorch; build it with `python vit-engine-cuda_b200/build.py`"
                                   ) from e
             entries = (_lib.lib.vitb200_quantize_fp8, _lib.lib.vitb200_layernorm_fp8,
-                       _lib.lib.vitb200_gemm_fp8, _lib.lib.vitb200_cross_attention)
+                       _lib.lib.vitb200_gemm_fp8, _lib.lib.vitb200_cross_attention,
+                       _lib.lib.vitb200_cross_attention_workspace_bytes)
             _serving.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in entries), _raise_status)
             _ops = _serving
     return _ops
