@@ -30,7 +30,6 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <limits>
 #include <type_traits>
 
 #include "cross_attention.cuh"
@@ -572,10 +571,7 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   a.lens = p.lens;
   a.o = static_cast<uint16_t*>(p.o);
   a.o_row = static_cast<int64_t>(p.heads) * D;
-  a.c = p.scale * kLog2e;
-  // Masked scores are infinite, and infinity times zero is NaN: the smallest
-  // float instead moves no score by more than 5e-7.
-  if (a.c == 0.f) a.c = std::numeric_limits<float>::denorm_min();
+  a.c = cross_scale(p.scale);
   a.err = device_error_word();
   // Pack a key head's G query heads into its row tiles; groups too large for a
   // tile (or that would waste half of one) run head by head, every query head
@@ -644,12 +640,20 @@ int cross_attention_prepare_device() {
       });
       if (st) return st;
     }
+  if (int st = cross_attention_rows_prepare_device()) return st;
   return cross_attention_token_prepare_device();
 }
 
 namespace {
 bool token_form(const CrossProblem& p) {
   return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows;
+}
+// Up to here the 64-row form is the faster one: 32 images x 12 heads x 577 keys,
+// D = 64, with 61, 128, 256 rows a head took 26, 38, 65 us, the tcgen05 form 39, 42,
+// 53; 16 x 4 heads of 256 rows x 1024 keys, D = 128, 35 and 26.
+constexpr int kRowsFormMost = 128;
+bool rows_form(const CrossProblem& p) {
+  return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kRowsFormMost;
 }
 }  // namespace
 
@@ -659,6 +663,7 @@ size_t cross_attention_workspace(const CrossProblem& p) {
 
 int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
   if (token_form(p)) return cross_attention_token_launch(p, s);
+  if (rows_form(p)) return cross_attention_rows_launch(p, s);
   return with_head(p.type, p.D, [&](auto tag, auto d) {
     return launch_tiles<decltype(tag), d.value>(p, s);
   });

@@ -1,9 +1,13 @@
-// Shared by the two forms of cross_attention (cross_attention.cu: row tiles on
-// tcgen05; cross_attention_token.cu: up to 16 rows per key head).
+// Shared by the three forms of cross_attention (cross_attention.cu: 128-row tiles
+// on tcgen05; cross_attention_rows.cu: 64-row tiles; cross_attention_token.cu: up to
+// 16 rows per key head).
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <limits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "engine.h"
@@ -14,6 +18,13 @@ namespace vitb200 {
 constexpr int kCrossMaxSplit = 8;  // CTAs that share an item's keys: a portable cluster
 constexpr int kTokenRows = 16;     // rows per key head the token form takes
 constexpr float kLog2e = 1.44269504088896340736f;
+
+// The softmax scale in log2 units. Masked scores are infinite, and infinity times
+// zero is NaN: the smallest float in place of zero moves no score by more than 5e-7.
+inline float cross_scale(float scale) {
+  const float c = scale * kLog2e;
+  return c == 0.f ? std::numeric_limits<float>::denorm_min() : c;
+}
 
 struct CrossTokenArgs {
   const uint16_t* q;
@@ -28,6 +39,9 @@ struct CrossTokenArgs {
   float c;     // scale * log2(e)
   int64_t q_row, q_batch, k_row, k_batch, v_row, v_batch, o_row;
 };
+int cross_attention_rows_prepare_device();
+int cross_attention_rows_launch(const CrossProblem& p, cudaStream_t s);
+
 int cross_attention_token_prepare_device();
 // Bytes of workspace its launch needs (0 where a CTA per key head does).
 size_t cross_attention_token_workspace(const CrossProblem& p);
@@ -63,6 +77,31 @@ __device__ __forceinline__ float4 ld_partial4(uint32_t addr, bool remote) {
                : "r"(addr)
                : "memory");
   return v;
+}
+
+// D += A B of one warp: 16 x 16 by 16 x 8, fp32 sums.
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                            uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The two values of a packed pair.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t p) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __half22float2(*reinterpret_cast<const __half2*>(&p));
+  else
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
 }
 
 // Sixteen bytes from global to shared memory, past L1; zeros where `inside` is

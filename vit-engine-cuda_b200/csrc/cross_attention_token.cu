@@ -60,21 +60,6 @@ struct TokenCfg {
   static constexpr int kRingBytes = kStages * kPieces<D> * 16 * kThreads;
 };
 
-template <typename T>
-__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                            uint32_t b1) {
-  if constexpr (std::is_same_v<T, __half>)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-        "{%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // The 8 x 8 matrix of 16-bit values a warp holds as fragments, transposed.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t t;
@@ -84,15 +69,6 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
-// The two values of a packed pair.
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t p) {
-  if constexpr (std::is_same_v<T, __half>)
-    return __half22float2(*reinterpret_cast<const __half2*>(&p));
-  else
-    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
 }
 
 // Floats of a warp's or CTA's partial result: [rows][D + 4], then m and l, rounded
@@ -569,18 +545,23 @@ int token_smem(int rows) {
 }
 
 // CTAs per key head of the streaming form for this problem, or 0 where a CTA per
-// image and key head does. Streaming spreads the steps evenly but finds its place in
-// the list and launches a second kernel (some 4 us): it is taken where the emptiest
-// SM would otherwise idle for longer, which at 40 GB/s an SM is 160 KB of keys and
-// values.
+// image and key head does. An SM reads 46 GB/s and the GPU 5.2 TB/s here; streaming
+// spreads the steps evenly, but finding its place in the list, further ramps and the
+// second kernel cost some 12 us. Both sides measured: 32 images x 8 heads x 2048
+// keys, D = 128, 55 us with a CTA each and 68 streaming; 2 x 8 x 32768, 367 and 66.
 template <int D>
 int stream_ctas(int B, int kv_heads, int Tk) {
-  constexpr int kPerSm = TokenCfg<D>::kPerSm;
   const int64_t items = static_cast<int64_t>(B) * kv_heads;
-  const int64_t slots = static_cast<int64_t>(device_num_sms()) * kPerSm;
+  const int64_t sms = device_num_sms();
+  const int64_t slots = sms * TokenCfg<D>::kPerSm;
   const int64_t steps = (static_cast<int64_t>(Tk) + kStep - 1) / kStep;
-  const int64_t idle = (items + slots - 1) / slots * steps - items * steps / slots;
-  if (idle * kStep * D * 4 * kPerSm <= 160 * 1024) return 0;
+  const double bytes = static_cast<double>(steps) * kStep * D * 4;  // of an image's key head
+  const double waves = static_cast<double>((items + slots - 1) / slots);
+  const double per_sm =
+      static_cast<double>(std::min<int64_t>(TokenCfg<D>::kPerSm, (items + sms - 1) / sms));
+  const double alone_us = waves * bytes * per_sm / 46e3;
+  const double stream_us = static_cast<double>(items) * bytes / 5.2e6 + 12.0;
+  if (alone_us <= stream_us) return 0;
   if (B * steps > INT32_MAX) return 0;  // the list is counted in 32 bits
   // A step a warp at least: the parts that are joined later cost time too.
   return static_cast<int>(std::min(slots / kv_heads, B * steps / TokenCfg<D>::kWarps));
