@@ -806,6 +806,32 @@ int allow_smem(Kernel kernel, int bytes) {
 
 constexpr int kMaxSplit = 8;  // portable cluster size
 
+// The K split that makes a launch of the tile kernel shortest: 0.27 us a K block
+// with 64 columns and 0.34 with 128, and for joining a cluster's sums 0.8 us, 0.1 a
+// CTA and up to 1.5 for a full tile's rows (fitted to splits 1..8 of eight shapes; 8
+// x 4096 x 4096 takes 12.1, 8.5 us with 64 columns split 1, 2 ways and 8.9, 7.0 with
+// 128 split 2, 4 ways; 577 x 1024 x 1024 5.9 and 10.5, 7.0 and 11.1). Only splits whose clusters
+// all fit the GPU at once: the others run a second wave (64 x 4096 x 1024, 64
+// columns, 16 clusters of 8: 10.7 us, of 4: 6.1).
+struct TilePlan {
+  int ksplit;
+  double us;
+};
+template <typename T, int BN>
+TilePlan plan_tile(int64_t tiles, int num_kb, int64_t M) {
+  const int sms = device_num_sms();
+  const double block_us = BN == 64 ? 0.27 : 0.34;
+  TilePlan best = {1, static_cast<double>((tiles + sms - 1) / sms) * num_kb * block_us};
+  for (int d = 2; d <= std::min(kMaxSplit, num_kb) && tiles * d <= sms; ++d) {
+    const double us = (num_kb + d - 1) / d * block_us + 0.8 + 0.1 * d +
+                      1.5 * static_cast<double>(std::min<int64_t>(M, kBM)) / kBM;
+    if (us < best.us && cluster_slots(gemm_fp8_tile_kernel<T, BN>, TileCfg<BN>::kSmem, kThreads,
+                                      d) >= tiles)
+      best = {d, us};
+  }
+  return best;
+}
+
 }  // namespace
 
 int gemm_fp8_prepare_device() {
@@ -837,20 +863,17 @@ int gemm_fp8_launch(const Fp8GemmProblem& p, cudaStream_t s) {
   a.gelu = p.gelu;
   a.vec_xs = aligned(p.xs, p.ldxs * 4, 16);
   a.err = device_error_word();
-  const int sms = device_num_sms();
   const int64_t pair_tiles = (p.M + 2 * kBM - 1) / (2 * kBM) * ((p.N + kPairBN - 1) / kPairBN);
   const int64_t m_tiles = (p.M + kBM - 1) / kBM;
-  const int64_t tiles128 = m_tiles * ((p.N + 127) / 128);
-  const int64_t tiles64 = m_tiles * ((p.N + 63) / 64);
+  const int64_t tiles64 = m_tiles * ((p.N + 63) / 64), tiles128 = m_tiles * ((p.N + 127) / 128);
   if (std::max(pair_tiles, tiles64) > INT32_MAX / kMaxSplit) return VITB200_E_UNSUPPORTED;
   return with_out_type(p.out_type, [&](auto tag) {
     using T = decltype(tag);
-    if (tiles128 > sms) return launch_pair<T>(p, a, s);
-    const bool narrow = 2 * tiles64 <= sms;
-    const int64_t tiles = narrow ? tiles64 : tiles128;
-    const int split = static_cast<int>(
-        std::max<int64_t>(1, std::min<int64_t>({sms / tiles, a.num_kb, kMaxSplit})));
-    return narrow ? launch_tile<T, 64>(p, a, split, s) : launch_tile<T, 128>(p, a, split, s);
+    if (tiles128 > device_num_sms()) return launch_pair<T>(p, a, s);
+    const TilePlan narrow = plan_tile<T, 64>(tiles64, a.num_kb, p.M);
+    const TilePlan wide = plan_tile<T, 128>(tiles128, a.num_kb, p.M);
+    return narrow.us <= wide.us ? launch_tile<T, 64>(p, a, narrow.ksplit, s)
+                                : launch_tile<T, 128>(p, a, wide.ksplit, s);
   });
 }
 
