@@ -248,72 +248,94 @@ __global__ void __launch_bounds__(kThreads, 1)
           drain_wait_x(&v_full[s], ((v_issued - 1 - s) / C::kVSlots) & 1, err);
     } else if (warp == 1 && nk > 0 && elect_one()) {
       // -------------------------------------------------------------- MMA
+      // One thread issues everything, and its own instructions between products of
+      // 64 cycles show: loops are unrolled, ring positions are counters, and a tile's
+      // barriers are waited on once. SHARED: two units (streams) per key tile.
       constexpr uint32_t kIdescS = idesc<T>(kKeys, false);
       constexpr uint32_t kIdescPV = idesc<T>(D, true);
-      const uint32_t q0 = smem_addr(sq), k0 = smem_addr(sk), v0 = smem_addr(sv);
-      auto key_tile = [&](int u) { return shared_keys ? u >> 1 : u; };
-      auto issue_s = [&](int u) -> bool {
-        const int i = u & 1, j = key_tile(u), s = j % C::kKSlots;
-        if (!mbar_wait(&k_full[s], (j / C::kKSlots) & 1, err, kErrWaitFull)) return false;
-        tc_fence_after();
-        const uint32_t qa = q0 + (shared_keys ? i * C::kTile : 0);
-        const uint32_t ka = k0 + s * C::kTile;
-#pragma unroll
-        for (int h = 0; h < C::kHalves; ++h) {
-          const uint64_t dq = make_sdesc_kmajor(qa + h * kHalfBytes, 128);
-          const uint64_t dk = make_sdesc_kmajor(ka + h * kHalfBytes, 128);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)  // 16 columns = 32 bytes = +2
-            umma_f16(tmem + i * kKeys, dq + 2 * kk, dk + 2 * kk, kIdescS, h + kk ? 1u : 0u);
-        }
-        umma_commit(&s_full[i]);
-        if (!shared_keys || i == 1) umma_commit(&k_empty[s]);  // the tile's last use
-        return true;
-      };
-      auto issue_pv = [&](int u) -> bool {
-        const int i = u & 1, n = u >> 1, j = key_tile(u), s = j % C::kVSlots;
-        if (!mbar_wait(&v_full[s], (j / C::kVSlots) & 1, err, kErrWaitFull)) return false;
-        const bool last = j0 + j == all - 1;
-        if (last && fix_tail && !mbar_wait(&tail_bar, 0, err, kErrWaitFull)) return false;
-        const uint32_t d = tmem + 2 * kKeys + i * D;
-        const uint32_t p = tmem + i * kKeys;
-        const uint64_t dv = sdesc_nmajor(v0 + s * C::kTile, kHalfBytes);
-        const int steps = last ? (tail_keys + 15) / 16 : kKeys / 16;
-        // The first half of the keys while the exponentials of the second run.
-        if (!mbar_wait(&p_half[i], n & 1, err, kErrWaitAccFull)) return false;
-        tc_fence_after();
-        // 16 keys a product: 2048 bytes of V, 8 columns of P. The full tile is
-        // unrolled: one thread issues every product, and a loop's own instructions
-        // between products of 64 cycles show.
-        if (steps == 8) {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, kk ? 1u : (n ? 1u : 0u));
-          if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+      const uint64_t dq0 = make_sdesc_kmajor(smem_addr(sq), 128);
+      const uint64_t dk0 = make_sdesc_kmajor(smem_addr(sk), 128);
+      const uint64_t dv0 = sdesc_nmajor(smem_addr(sv), kHalfBytes);
+      constexpr uint64_t kTileStep = C::kTile >> 4, kHalfStep = kHalfBytes >> 4;
+      auto run = [&](auto shared) {
+        constexpr bool SHARED = decltype(shared)::value;
+        int ks = 0, vs = 0;           // ring positions
+        uint32_t kph = 0, vph = 0;    // and their phases
+        auto issue_s = [&](int i) -> bool {
+          if ((!SHARED || i == 0) && !mbar_wait(&k_full[ks], kph, err, kErrWaitFull)) return false;
           tc_fence_after();
+          const uint64_t dq = dq0 + (SHARED && i ? kTileStep : 0);
+          const uint64_t dk = dk0 + static_cast<uint32_t>(ks) * kTileStep;
+          const uint32_t d = tmem + i * kKeys;
 #pragma unroll
-          for (int kk = 4; kk < 8; ++kk)
-            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
-        } else {
-          for (int kk = 0; kk < min(4, steps); ++kk)
-            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
-          if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+          for (int h = 0; h < C::kHalves; ++h)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)  // 16 columns = 32 bytes = +2
+              umma_f16(d, dq + h * kHalfStep + 2 * kk, dk + h * kHalfStep + 2 * kk, kIdescS,
+                       h + kk ? 1u : 0u);
+          umma_commit(&s_full[i]);
+          if (!SHARED || i == 1) {  // the tile's last use
+            umma_commit(&k_empty[ks]);
+            if (++ks == C::kKSlots) ks = 0, kph ^= 1u;
+          }
+          return true;
+        };
+        auto issue_pv = [&](int i, int n, bool last) -> bool {
+          if (!SHARED || i == 0) {
+            if (!mbar_wait(&v_full[vs], vph, err, kErrWaitFull)) return false;
+            if (last && fix_tail && !mbar_wait(&tail_bar, 0, err, kErrWaitFull)) return false;
+          }
+          const uint64_t dv = dv0 + static_cast<uint32_t>(vs) * kTileStep;
+          const uint32_t d = tmem + 2 * kKeys + i * D;
+          const uint32_t p = tmem + i * kKeys;
+          // The first half of the keys while the exponentials of the second run; 16
+          // keys a product: 2048 bytes of V, 8 columns of P.
+          if (!mbar_wait(&p_half[i], n & 1, err, kErrWaitAccFull)) return false;
           tc_fence_after();
-          for (int kk = 4; kk < steps; ++kk)
-            umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+          const int steps = last ? (tail_keys + 15) / 16 : kKeys / 16;
+          if (steps == 8) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, kk ? 1u : (n ? 1u : 0u));
+            if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk)
+              umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+          } else {
+            for (int kk = 0; kk < min(4, steps); ++kk)
+              umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, n || kk ? 1u : 0u);
+            if (!mbar_wait(&p_full[i], n & 1, err, kErrWaitAccFull)) return false;
+            tc_fence_after();
+            for (int kk = 4; kk < steps; ++kk)
+              umma_f16_tmem_a(d, p + 8 * kk, dv + 128 * kk, kIdescPV, 1u);
+          }
+          umma_commit(&pv_done[i]);
+          if (!SHARED || i == 1) {
+            umma_commit(&v_empty[vs]);
+            if (++vs == C::kVSlots) vs = 0, vph ^= 1u;
+          }
+          return true;
+        };
+        bool ok = mbar_wait(&q_full, 0, err, kErrWaitFull);
+        // S(u + 2) overwrites P(u): it is issued after the product that reads P(u),
+        // and one thread's products run in order.
+        if (ok) ok = issue_s(0);
+        if (ok && units > 1) ok = issue_s(1);
+        for (int u = 0; u < units && ok; u += 2) {
+          const int n = u >> 1;
+          const int j = j0 + (SHARED ? n : u);  // key tile of unit u
+          ok = issue_pv(0, n, j == all - 1);
+          if (ok && u + 2 < units) ok = issue_s(0);
+          if (!ok || u + 1 >= units) break;
+          ok = issue_pv(1, n, (SHARED ? j : j + 1) == all - 1);
+          if (ok && u + 3 < units) ok = issue_s(1);
         }
-        umma_commit(&pv_done[i]);
-        if (!shared_keys || i == 1) umma_commit(&v_empty[s]);
-        return true;
       };
-      bool ok = mbar_wait(&q_full, 0, err, kErrWaitFull);
-      // S(u + 2) overwrites P(u): it is issued after the product that reads P(u),
-      // and one thread's products run in order.
-      for (int u = 0; u < 2 && u < units && ok; ++u) ok = issue_s(u);
-      for (int u = 0; u < units && ok; ++u) {
-        ok = issue_pv(u);
-        if (ok && u + 2 < units) ok = issue_s(u + 2);
-      }
+      if (shared_keys)
+        run(std::true_type{});
+      else
+        run(std::false_type{});
       umma_commit(&mma_done);
       drain_wait_x(&mma_done, 0, err);
     } else if (warp == 2 && fix_tail) {
@@ -353,12 +375,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int n = 0; n < mine; ++n) {
       const int j = j0 + (shared_keys ? n : 2 * n + i);
-      if (!warp_wait_x(&s_full[i], n & 1, err, kErrWaitAccFull, lane)) {
-        ok = false;
-        break;
-      }
-      // S(n) was issued after the stream's product n - 1: that one is in O.
-      if (n > 0 && !warp_wait_x(&pv_done[i], (n - 1) & 1, err, kErrWaitAccFull, lane)) {
+      // Every lane waits: that is quicker than one lane and a broadcast. S(n) was
+      // issued after the stream's product n - 1, so that one is in O as well.
+      ok = mbar_wait(&s_full[i], n & 1, err, kErrWaitAccFull) &&
+           (n == 0 || mbar_wait(&pv_done[i], (n - 1) & 1, err, kErrWaitAccFull));
+      if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
