@@ -42,11 +42,6 @@ namespace {
 constexpr int kRows = 128;       // rows of a tile
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kThreads = 384;    // control warpgroup + two softmax warpgroups
-// 384 threads launched at 168 registers: 128 * 56 + 256 * 224 = 384 * 168
-// (build.py checks that ptxas allocated 168).
-constexpr uint32_t kCtrlRegs = 56;
-constexpr uint32_t kSoftRegs = 224;
-static_assert(128 * kCtrlRegs + 256 * kSoftRegs == kThreads * 168, "register split");
 constexpr int kHalf = 64;                        // columns of one 128-byte swizzle span
 constexpr int kHalfBytes = kRows * kHalf * 2;    // 128 rows x 64 columns
 constexpr float kRescale = 8.f;                  // log2 of the largest P
@@ -58,6 +53,13 @@ struct Cfg {
   static constexpr int kKSlots = D == 64 ? 4 : 2;
   static constexpr int kVSlots = D == 64 ? 4 : 3;
   static constexpr int kSmem = (2 + kKSlots + kVSlots) * kTile + 1024;
+  // 384 threads launched at 168 registers (build.py checks that ptxas allocated
+  // 168), shared out between control and softmax warpgroups. D = 128 waits on the
+  // issuing thread, which spills below 104 (503 us against 488 at 4 x 16 heads x
+  // 4096 x 4500); D = 64 on the softmax (421 against 446 at 4 x 16 x 4096 x 4096).
+  static constexpr uint32_t kCtrlRegs = D == 64 ? 56 : 104;
+  static constexpr uint32_t kSoftRegs = D == 64 ? 224 : 200;
+  static_assert(128 * kCtrlRegs + 256 * kSoftRegs == kThreads * 168, "register split");
   // Partial results of both streams, joined at the end: [2][128][D + 4] floats
   // (the pad keeps a thread-per-row store free of bank conflicts), then m and l.
   static constexpr int kPitch = D + 4;
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool fix_tail = nk > 0 && j0 + nk == all && len < a.Tk && tail_keys < kKeys;
 
   if (warp < 4) {
-    setmaxnreg_dec<kCtrlRegs>();
+    setmaxnreg_dec<C::kCtrlRegs>();
     if (warp == 0 && nk > 0 && elect_one()) {
       // -------------------------------------------------------------- TMA
       mbar_arrive_expect_tx(&q_full, static_cast<uint32_t>(it.tiles * C::kHalves * a.group *
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Softmax state of this thread's row, kept past the role split.
   const bool joined = a.nsplit > 1 || !shared_keys;  // rows have several partial results
   if (warp >= 4) {
-    setmaxnreg_inc<kSoftRegs>();
+    setmaxnreg_inc<C::kSoftRegs>();
     // ---------------------------------------------------------------- softmax
     const int i = (warp - 4) >> 2;  // stream
     const int quarter = warp & 3;
