@@ -671,12 +671,16 @@ namespace {
 bool token_form(const CrossProblem& p) {
   return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows;
 }
-// Up to here the 64-row form is the faster one: 32 images x 12 heads x 577 keys,
-// D = 64, with 61, 128, 256 rows a head took 26, 38, 65 us, the tcgen05 form 39, 42,
-// 53; 16 x 4 heads of 256 rows x 1024 keys, D = 128, 35 and 26.
-constexpr int kRowsFormMost = 128;
+// The 64-row form is the faster one for up to 128 rows (32 images x 12 heads x 577
+// keys, D = 64, with 61, 128, 256 rows a head took 26, 38, 65 us, the tcgen05 form
+// 39, 42, 46; 16 x 4 heads of 256 rows x 1024 keys, D = 128, 35 and 26), and for so
+// few keys that a CTA's set-up is most of its work (25 x 12 heads of 2224 rows, D =
+// 64: 64 keys 80 against 134 us, 128 keys 109 and 124, 200 keys 178 and 164; 8 x 16
+// heads of 1024 rows, D = 128: 64 keys 36 and 40, 130 keys 61 and 46).
 bool rows_form(const CrossProblem& p) {
-  return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kRowsFormMost;
+  const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq;
+  if (rows > INT32_MAX / 2) return false;  // counted in 32 bits there
+  return rows <= 128 || p.Tk <= (p.D == 64 ? 128 : 64);
 }
 }  // namespace
 

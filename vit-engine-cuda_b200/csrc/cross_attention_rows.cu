@@ -230,6 +230,9 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
   }
   copy_async_wait<0>();
 
+  // (Stored as they lie in registers: through shared memory, in 16-byte pieces, the
+  // rows' addresses cost more than the wider stores save, 88 against 80 us at 300
+  // heads of 2224 rows.)
   if (a.nsplit == 1) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
