@@ -621,12 +621,14 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
                               static_cast<uint64_t>(a.kv_heads), static_cast<uint64_t>(p.B)};
     const uint64_t strides[4] = {D * es, static_cast<uint64_t>(p.q_row) * es,
                                  static_cast<uint64_t>(a.group) * D * es,
-                                 static_cast<uint64_t>(p.q_batch) * es};
+                                 static_cast<uint64_t>(p.B == 1 ? p.q_row * p.Tq : p.q_batch) * es};
     const uint32_t box[5] = {kHalf, static_cast<uint32_t>(a.group),
                              static_cast<uint32_t>(a.tile_t), 1, 1};
     if (int st = encode_tmap_typed(&tq, 5, p.q, dims, strides, box, 1, 1)) return st;
   }
+  // (One image has no batch stride; a map wants a real one.)
   auto kv_map = [&](CUtensorMap* map, const void* t, int64_t row, int64_t batch) {
+    if (p.B == 1) batch = row * p.Tk;
     const uint64_t dims[4] = {D, static_cast<uint64_t>(p.Tk), static_cast<uint64_t>(p.kv_heads),
                               static_cast<uint64_t>(p.B)};
     const uint64_t strides[3] = {static_cast<uint64_t>(row) * es, D * es,
