@@ -105,10 +105,13 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// 128 x 128 blocks: a CTA holds a block, in its own type until it is coded.
+// 128 x 128 blocks: a CTA holds a block, in its own type until it is coded. Loads,
+// maximum and stores overlap only between CTAs, so as many as fit share an SM (4096 x
+// 4096 bf16: 12.4 us, 4.1 TB/s, with three of 512 threads; 12.8 with two, 17 with
+// five of 256).
 constexpr int kBlockThreads = 512;
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(kBlockThreads, 2)
+__global__ void __launch_bounds__(kBlockThreads, sizeof(T) == 2 ? 3 : 2)
     quantize_blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int kb,
                            uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scales,
                            int64_t blocks) {
