@@ -106,12 +106,14 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // 128 x 128 blocks: a CTA holds a block, in its own type until it is coded. Loads,
-// maximum and stores overlap only between CTAs, so as many as fit share an SM (4096 x
-// 4096 bf16: 12.4 us, 4.1 TB/s, with three of 512 threads; 12.8 with two, 17 with
-// five of 256).
+// maximum and stores overlap only between CTAs. Three an SM for 16-bit rows read in 16-byte
+// pieces: 4096 x 4096 bf16 12.4 us, 4.1 TB/s, against 12.8 with two or four CTAs and
+// 17 with 256 threads (768 x 768, less than a block an SM: 2.6 against 2.3). Rows
+// read value by value spill with three, 4096 x 4095 19.1 us against 15.4. A thread
+// holds 32 registers of an fp32 block, so two (4096 x 4096: 17.6 us).
 constexpr int kBlockThreads = 512;
 template <typename T, int ROWS>
-__global__ void __launch_bounds__(kBlockThreads, sizeof(T) == 2 ? 3 : 2)
+__global__ void __launch_bounds__(kBlockThreads, sizeof(T) == 2 && ROWS != kScalarRows ? 3 : 2)
     quantize_blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, int K, int kb,
                            uint8_t* __restrict__ q, int64_t ldq, float* __restrict__ scales,
                            int64_t blocks) {
