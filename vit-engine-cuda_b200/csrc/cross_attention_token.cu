@@ -8,8 +8,8 @@
 // m16n8k16, with keys (then output columns) as the product's 16 rows and eight query
 // rows as its columns, with its own running maxima, sums and output, and no barrier
 // until the end. (The legacy tensor path is far from its limit at one product or two
-// per loaded fragment; query rows as the product's 16 rows took twice the products
-// and registers, and ran at 4.2 TB/s.)
+// per loaded fragment; query rows as the product's 16 rows take twice the products
+// and registers.)
 //  * S^T = K Q^T: a lane's 16-byte load is eight neighbouring columns of one key.
 //    The order in which the columns enter the sum is free, so these eight serve as
 //    fragments of two products, with Q's fragments loaded in the same order.
@@ -24,8 +24,8 @@
 // key head, which as many CTAs as the head gets cut into equal parts, whatever the
 // images' lengths: the parts of an image that several CTAs share go to a workspace,
 // and a second kernel adds them in order. Neighbouring CTAs take the same part for
-// neighbouring heads, whose keys lie side by side: one list of all heads instead
-// reads 256-byte pieces far apart, at 4.2 TB/s. (Sharing a key head over a cluster
+// neighbouring heads, whose keys lie side by side: one list of all heads would
+// read 256-byte pieces far apart. (Sharing a key head over a cluster
 // needs no workspace, but 16 clusters of 8 one-per-SM CTAs do not fit the GPU at
 // once, and images of different lengths finish at different times: 2 x 8 heads x
 // 32768 keys ran at 2.6 TB/s.)
@@ -545,7 +545,7 @@ int token_smem(int rows) {
 }
 
 // CTAs per key head of the streaming form for this problem, or 0 where a CTA per
-// image and key head does. An SM reads 46 GB/s and the GPU 5.2 TB/s here; streaming
+// image and key head does. Fitted: an SM reads 46 GB/s, the GPU 5.2 TB/s; streaming
 // spreads the steps evenly, but finding its place in the list, further ramps and the
 // second kernel cost some 12 us. Both sides measured: 32 images x 8 heads x 2048
 // keys, D = 128, 55 us with a CTA each and 68 streaming; 2 x 8 x 32768, 367 and 66.

@@ -6,7 +6,8 @@ block of 128 (``gemm_fp8``) and attention to an encoder's states of another leng
 They keep the manner of ``vit_cuda._C``: CUDA tensors on the current device
 (RuntimeError otherwise), fresh outputs from PyTorch's caching allocator, work
 launched asynchronously on the current stream, scratch space from the caching
-allocator too, so that they can be captured in a CUDA graph. They are forward only, like every op of this package.
+allocator too, so that they can be captured in a CUDA graph. They are forward
+only, like every op of this package.
 
 The checks and the call into libvitb200.so are compiled (csrc/bindings.cpp, built
 as ``vit_cuda._serving``): in a single token's step the host's time per call is
