@@ -12,7 +12,12 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/DispatchKeySet.h>
+#include <c10/core/GradMode.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -115,6 +120,41 @@ bool passed(int status, const char* what) {
   Py_XDECREF(r);
   if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, what);
   return false;
+}
+
+// Whether somebody looks on: a tracer, a dispatch or function mode, a transform
+// (vmap, functionalize), or gradients. The functions below read memory behind the
+// dispatcher's back, so such a call has to go to the registered operator instead.
+bool watched_thread() {
+  // BackendSelect and the like are always included, autocast's keys change nothing here
+  const c10::DispatchKeySet keys = c10::impl::tls_local_dispatch_key_set().included_ -
+                                   c10::default_included_set - c10::autocast_dispatch_keyset;
+  return !keys.empty() || c10::impl::dispatch_mode_enabled() ||
+         at::impl::torch_function_mode_enabled();
+}
+bool watched_arg(PyObject* o) {
+  if (o == Py_None) return false;
+  if (!THPVariable_CheckExact(o)) {  // a subclass or a proxy; anything else is refused later
+    return THPVariable_Check(o) || PyObject_HasAttrString(o, "__torch_function__");
+  }
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (c10::GradMode::is_enabled() && t.requires_grad()) return true;
+  TORCH_CHECK(!t._fw_grad(0).defined(), "vit_cuda: forward only, and an input has a tangent");
+  // anything but a plain CUDA tensor (CPU tensors are refused later): fakes, wrappers,
+  // views with a pending negation
+  const c10::DispatchKeySet keys = t.key_set() - c10::autograd_dispatch_keyset_with_ADInplaceOrView -
+                                   c10::autocast_dispatch_keyset;
+  return keys != c10::DispatchKeySet(c10::DispatchKey::CUDA) &&
+         keys != c10::DispatchKeySet(c10::DispatchKey::CPU);
+}
+
+// (tensors or None...) -> bool
+PyObject* watched(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  bool yes = watched_thread();
+  for (Py_ssize_t i = 0; i < n && !yes; ++i) yes = watched_arg(args[i]);
+  return PyBool_FromLong(yes);
+  END_HANDLE_TH_ERRORS
 }
 
 void check_count(Py_ssize_t n, Py_ssize_t want) {
@@ -354,9 +394,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define VITB200_METHOD(f) \
   {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {VITB200_METHOD(bind),          VITB200_METHOD(quantize_fp8),
-                          VITB200_METHOD(layernorm_fp8), VITB200_METHOD(gemm_fp8),
-                          VITB200_METHOD(cross_attention), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef kMethods[] = {VITB200_METHOD(bind),         VITB200_METHOD(watched),
+                          VITB200_METHOD(quantize_fp8), VITB200_METHOD(layernorm_fp8),
+                          VITB200_METHOD(gemm_fp8),     VITB200_METHOD(cross_attention),
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, kMethods};
 
 }  // namespace

@@ -3,7 +3,9 @@ project's drop-in surface: the eight ops of ``vit_cuda._C`` re-exported as
 ``vit_cuda.<op>`` (the reference tests call them that way, e.g.
 tests/test_qkv.py:37) and ``vit_cuda.model.ViTCUDA``. The ``vit_cuda.<op>``
 names go through ``torch.ops.vit_cuda.<op>`` (registered custom ops that
-``torch.compile`` traces); ``vit_cuda._C.<op>`` calls the library directly.
+``torch.compile`` traces); ``vit_cuda._C.<op>`` calls the library directly. The
+serving operators (``vit_cuda.serving``) do so by themselves where nothing traces
+or differentiates.
 """
 from . import _C
 from .library import (classifier_forward, cross_attention, flash_attn_2, gemm_bias, gemm_fp8,

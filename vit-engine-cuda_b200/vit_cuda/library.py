@@ -6,7 +6,8 @@ Every op of ``vit_cuda._C`` (csrc/bindings/binding.cpp:5-23 of the reference)
 becomes ``torch.ops.vit_cuda.<op>`` with a fake (shape-only) implementation for
 tracing; the CUDA implementation is the ``_C`` function itself. The public
 ``vit_cuda.<op>`` names call these registered ops; ``vit_cuda._C.<op>`` stays
-the direct call (no dispatcher), like the reference's pybind module.
+the direct call (no dispatcher), like the reference's pybind module. The serving
+operators are registered the same way.
 
 Two adaptations to the custom-op rules (outputs may not alias each other):
 ``qkv_proj`` is registered as ``qkv_proj_packed`` returning one ``[3, B, N, E]``
@@ -24,6 +25,7 @@ from typing import Optional
 import torch
 
 from . import _C, serving
+from .serving import cross_attention, gemm_fp8, layernorm_fp8, quantize_fp8  # noqa: F401
 
 
 # ---------------------------------------------------------------- ops
@@ -116,8 +118,8 @@ def _(X, W, B):
 
 
 # ---------------------------------------------------------------- serving ops
-# vit_cuda.<op> calls these only while torch.compile traces; an eager call goes
-# straight to vit_cuda.serving, without the dispatcher's tens of microseconds.
+# vit_cuda.<op> (vit_cuda/serving.py) calls these where something traces, transforms or
+# differentiates; a plain call goes past the dispatcher and its tens of microseconds.
 def _fake_codes(X):
     K = X.shape[-1]
     ld = (K + 15) // 16 * 16
@@ -127,7 +129,7 @@ def _fake_codes(X):
 
 @torch.library.custom_op("vit_cuda::quantize_fp8", mutates_args=())
 def _quantize_fp8(X: torch.Tensor, block_rows: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return serving.quantize_fp8(X, block_rows)
+    return serving.direct().quantize_fp8(X, block_rows)
 
 
 @_quantize_fp8.register_fake
@@ -140,7 +142,7 @@ def _(X, block_rows):
 @torch.library.custom_op("vit_cuda::layernorm_fp8", mutates_args=())
 def _layernorm_fp8(X: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
                    eps: float) -> tuple[torch.Tensor, torch.Tensor]:
-    return serving.layernorm_fp8(X, gamma, beta, eps)
+    return serving.direct().layernorm_fp8(X, gamma, beta, eps)
 
 
 @_layernorm_fp8.register_fake
@@ -153,7 +155,7 @@ def _(X, gamma, beta, eps):
 def _gemm_fp8(X: torch.Tensor, X_scale: torch.Tensor, W: torch.Tensor, W_scale: torch.Tensor,
               B: Optional[torch.Tensor], residual: Optional[torch.Tensor], gelu: bool,
               out_dtype: torch.dtype) -> torch.Tensor:
-    return serving.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+    return serving.direct().gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
 
 
 @_gemm_fp8.register_fake
@@ -164,7 +166,7 @@ def _(X, X_scale, W, W_scale, B, residual, gelu, out_dtype):
 @torch.library.custom_op("vit_cuda::cross_attention", mutates_args=())
 def _cross_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, scale: float, heads: int,
                      kv_heads: Optional[int], kv_lens: Optional[torch.Tensor]) -> torch.Tensor:
-    return serving.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+    return serving.direct().cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
 
 
 @_cross_attention.register_fake
@@ -229,31 +231,3 @@ def qkv_proj(X, W, B):
 
 def gemm_bias(X, W, B):
     return torch.ops.vit_cuda.gemm_bias(X, W, B)
-
-
-def quantize_fp8(X, block_rows=1):
-    if torch.compiler.is_compiling():
-        return torch.ops.vit_cuda.quantize_fp8(X, block_rows)
-    return serving.quantize_fp8(X, block_rows)
-
-
-def layernorm_fp8(X, gamma, beta, eps):
-    if torch.compiler.is_compiling():
-        return torch.ops.vit_cuda.layernorm_fp8(X, gamma, beta, eps)
-    return serving.layernorm_fp8(X, gamma, beta, eps)
-
-
-def gemm_fp8(X, X_scale, W, W_scale, B=None, residual=None, gelu=False, out_dtype=torch.float32):
-    if torch.compiler.is_compiling():
-        return torch.ops.vit_cuda.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
-    return serving.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
-
-
-def cross_attention(Q, K, V, scale, heads, kv_heads=None, kv_lens=None):
-    if torch.compiler.is_compiling():
-        return torch.ops.vit_cuda.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
-    return serving.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
-
-
-for _name in serving.__all__:
-    globals()[_name].__doc__ = getattr(serving, _name).__doc__

@@ -7,7 +7,12 @@ They keep the manner of ``vit_cuda._C``: CUDA tensors on the current device
 (RuntimeError otherwise), fresh outputs from PyTorch's caching allocator, work
 launched asynchronously on the current stream, scratch space from the caching
 allocator too, so that they can be captured in a CUDA graph. They are forward
-only, like every op of this package.
+only, like every op of this package: an output of inputs that require a gradient
+requires one too, and its backward raises.
+
+Each op is registered as ``torch.ops.vit_cuda.<op>`` (vit_cuda/library.py). A plain
+call goes past the dispatcher; one that a tracer, a dispatch or function mode, a
+transform or autograd has to see goes through the registered op.
 
 The checks and the call into libvitb200.so are compiled (csrc/bindings.cpp, built
 as ``vit_cuda._serving``): in a single token's step the host's time per call is
@@ -32,6 +37,11 @@ _lock = threading.Lock()
 
 def _raise_status(status: int, what: str) -> None:
     raise _lib.VitB200Error(what, status)
+
+
+def direct():
+    """The compiled module itself: what the registered ops run on the GPU."""
+    return _ops or _load()
 
 
 def _load():
@@ -63,14 +73,18 @@ def quantize_fp8(X: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
     128 x 128 of a 2-D X, scales [ceil(N/128), ceil(K/128)] (weights). Rows of the
     codes are 16 bytes or a multiple apart. A block holding a NaN or an infinity
     dequantises to NaN."""
-    return (_ops or _load()).quantize_fp8(X, block_rows)
+    if torch.compiler.is_compiling() or (_ops or _load()).watched(X):
+        return torch.ops.vit_cuda.quantize_fp8(X, block_rows)
+    return _ops.quantize_fp8(X, block_rows)
 
 
 def layernorm_fp8(X: torch.Tensor, gamma: torch.Tensor, beta: torch.Tensor,
                   eps: float) -> tuple[torch.Tensor, torch.Tensor]:
     """``quantize_fp8(layernorm_forward(X, gamma, beta, eps))`` in one pass over X
     [..., K] (float32, float16 or bfloat16; gamma and beta float32): (codes, scales)."""
-    return (_ops or _load()).layernorm_fp8(X, gamma, beta, eps)
+    if torch.compiler.is_compiling() or (_ops or _load()).watched(X, gamma, beta):
+        return torch.ops.vit_cuda.layernorm_fp8(X, gamma, beta, eps)
+    return _ops.layernorm_fp8(X, gamma, beta, eps)
 
 
 def gemm_fp8(X: torch.Tensor, X_scale: torch.Tensor, W: torch.Tensor, W_scale: torch.Tensor,
@@ -81,7 +95,10 @@ def gemm_fp8(X: torch.Tensor, X_scale: torch.Tensor, W: torch.Tensor, W_scale: t
     W_scale [ceil(N_out/128), ceil(K/128)]; B [N_out] float32, act erf-GELU when
     ``gelu``, residual of Y's shape and type. Sums are float32, Y is rounded once
     to ``out_dtype`` (float32, float16 or bfloat16)."""
-    return (_ops or _load()).gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+    if torch.compiler.is_compiling() or (_ops or _load()).watched(X, X_scale, W, W_scale, B,
+                                                                  residual):
+        return torch.ops.vit_cuda.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
+    return _ops.gemm_fp8(X, X_scale, W, W_scale, B, residual, gelu, out_dtype)
 
 
 def cross_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, scale: float, heads: int,
@@ -95,7 +112,9 @@ def cross_attention(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, scale: fl
     ``kv_lens`` [B] int32: the keys of each image, clamped to 0..Tk; keys past it
     may hold anything, and an image without keys gets zeros. K and V may be column
     ranges of one tensor (no copy is made)."""
-    return (_ops or _load()).cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+    if torch.compiler.is_compiling() or (_ops or _load()).watched(Q, K, V, kv_lens):
+        return torch.ops.vit_cuda.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
+    return _ops.cross_attention(Q, K, V, scale, heads, kv_heads, kv_lens)
 
 
 __all__ = ["quantize_fp8", "layernorm_fp8", "gemm_fp8", "cross_attention"]
