@@ -1,6 +1,6 @@
 """Builds libvitb200.so (the sm_100a kernels + C ABI) in-tree with nvcc, and
 _serving.so (csrc/bindings.cpp: the serving operators' Python entry points,
-compiled against the installed PyTorch) with g++.
+compiled against the installed PyTorch, and left out where there is none) with g++.
 
     python vit-engine-cuda_b200/build.py [--force] [--jobs N]
 
@@ -30,6 +30,7 @@ LIB = os.path.join(OUT_DIR, "libvitb200.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 BINDINGS = os.path.join(CSRC, "bindings.cpp")
 BINDINGS_LIB = os.path.join(OUT_DIR, "_serving.so")
+BINDINGS_STAMP = os.path.join(OBJ_DIR, "_serving.built_for")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -67,24 +68,48 @@ def up_to_date() -> bool:
     return newer_than(LIB, sources() + headers() + [__file__])
 
 
-def build_bindings(force: bool = False) -> str:
+def torch_package() -> str | None:
+    """PyTorch's directory, found without importing it; None where it is not installed."""
+    spec = importlib.util.find_spec("torch")
+    return spec.submodule_search_locations[0] if spec else None
+
+
+def built_for(torch_dir: str) -> str:
+    """The PyTorch that _serving.so is compiled against (its ABI differs by version)."""
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        return re.search(r"__version__ = ['\"](.*?)['\"]", f.read()).group(1)
+
+
+def build_bindings(force: bool = False) -> str | None:
+    torch_dir = torch_package()
+    if torch_dir is None:
+        print("PyTorch is not installed: libvitb200.so (the C ABI) is built without vit_cuda/"
+              "_serving.so, the serving operators' Python entry points", file=sys.stderr)
+        return None
     header = os.path.join(INCLUDE, "vitb200.h")
+    version = built_for(torch_dir)
+    # File times say nothing about the PyTorch and the interpreter they were built for.
+    stamp, wanted = BINDINGS_STAMP, f"{version}\n{sysconfig.get_config_var('EXT_SUFFIX')}\n"
     if not force and newer_than(BINDINGS_LIB, [BINDINGS, header, __file__]):
-        return BINDINGS_LIB
-    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+        if os.path.exists(stamp) and open(stamp).read() == wanted:
+            return BINDINGS_LIB
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     includes = [os.path.join(torch_dir, "include"),
                 os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                 os.path.join(cuda, "include"), sysconfig.get_paths()["include"], INCLUDE]
     tmp = BINDINGS_LIB + ".tmp"
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++20", "-fPIC", "-shared",
-           "-fvisibility=hidden", *(f"-I{d}" for d in includes), BINDINGS, "-o", tmp,
+           "-fvisibility=hidden", f'-DVITB200_BUILT_FOR="{version}"',
+           *(f"-I{d}" for d in includes), BINDINGS, "-o", tmp,
            f"-L{os.path.join(torch_dir, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
            "-ltorch_cuda", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {BINDINGS}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BINDINGS_LIB)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(wanted)
     return BINDINGS_LIB
 
 

@@ -402,4 +402,12 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_serving", nullptr, -1, kMethods}
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__serving(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__serving(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  // (a module of another PyTorch may still find all its symbols)
+  if (m && PyModule_AddStringConstant(m, "BUILT_FOR", VITB200_BUILT_FOR) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
