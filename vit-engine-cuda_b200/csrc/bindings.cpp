@@ -72,7 +72,8 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, c10::DeviceIndex de
 }
 
 // A tensor read as [rows, last dim]: as it is where one stride (in elements)
-// describes the rows, else a contiguous copy.
+// describes the rows, else a contiguous copy. The stride of a dimension of one means
+// nothing, so one token of each sequence ([B, 1, K]) goes by its batch stride.
 struct Rows {
   at::Tensor t;
   int64_t ld;
@@ -82,9 +83,12 @@ Rows rows_of(const at::Tensor& t) {
   if (t.is_contiguous()) return {t, n};
   if (t.stride(-1) == 1) {
     if (t.dim() == 2 && t.stride(0) >= n) return {t, t.stride(0)};
-    // a padded [B, N, K] still has one stride
-    if (t.dim() == 3 && t.stride(1) >= n && t.stride(0) == t.size(1) * t.stride(1))
-      return {t, t.stride(1)};
+    if (t.dim() == 3) {
+      const int64_t ld = t.size(1) == 1 ? t.stride(0) : t.stride(1);
+      // (a padded [B, N, K] still has one stride)
+      if (ld >= n && (t.size(0) == 1 || t.size(1) == 1 || t.stride(0) == t.size(1) * ld))
+        return {t, ld};
+    }
   }
   return {t.contiguous(), n};
 }
@@ -103,6 +107,8 @@ Rows empty_codes(at::IntArrayRef shape, c10::DeviceIndex device) {
 // rows_of codes, with rows and base aligned to 16 bytes (a padded copy if not).
 Rows code_rows(const at::Tensor& q, c10::DeviceIndex device) {
   Rows r = rows_of(q);
+  // One row counts as contiguous whatever its stride; nothing past it is read.
+  if (q.numel() == q.size(-1)) r.ld = (r.ld + 15) / 16 * 16;
   if (r.ld % 16 == 0 && reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0) return r;
   Rows c = empty_codes(q.sizes(), device);
   c.t.view(at::kByte).copy_(q.view(at::kByte));
