@@ -83,3 +83,11 @@ def test_python_refuses_cpu_tensors():
                  lambda: vit_cuda.cross_attention(x[None], x[None], x[None], 0.1, 2)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_quantisers_refuse_unaligned_fp32():
+    """An fp32 pointer off a 4-byte boundary would fault on the GPU."""
+    for off in (1, 2, 3):
+        assert quantize(scales=P + off) == layernorm(scales=P + off) == _lib.E_ALIGNMENT
+        assert layernorm(gamma=P + off) == layernorm(beta=P + off) == _lib.E_ALIGNMENT
+    assert layernorm(gamma=None, beta=P + 1) == _lib.E_INVALID_ARG

@@ -463,7 +463,8 @@ int check_quantize(const void* x, int type, int64_t rows, int K, int64_t ldx, co
   if (rows < 0 || K < 1 || K > (1 << 30) || ldx < K || ldq < K) return VITB200_E_INVALID_ARG;
   if (type < VITB200_F32 || type > VITB200_BF16) return VITB200_E_INVALID_ARG;
   if (ldq % 16 != 0 || reinterpret_cast<uintptr_t>(q) % 16 != 0) return VITB200_E_ALIGNMENT;
-  if (reinterpret_cast<uintptr_t>(x) % (type == VITB200_F32 ? 4 : 2) != 0)
+  if (reinterpret_cast<uintptr_t>(x) % (type == VITB200_F32 ? 4 : 2) != 0 ||
+      reinterpret_cast<uintptr_t>(scales) % 4 != 0)
     return VITB200_E_ALIGNMENT;
   if (rows == 0) return 1;
   return x && q && scales ? 0 : VITB200_E_INVALID_ARG;
@@ -491,6 +492,8 @@ extern "C" int vitb200_layernorm_fp8(const void* x, int x_type, int64_t rows, in
   try {
     if (int st = check_quantize(x, x_type, rows, K, ldx, q, ldq, scales)) return st > 0 ? 0 : st;
     if (!gamma || !beta) return VITB200_E_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(gamma) % 4 != 0 || reinterpret_cast<uintptr_t>(beta) % 4 != 0)
+      return VITB200_E_ALIGNMENT;
     if (int st = vitb200_init()) return st;
     return layernorm_fp8_launch(x, x_type, rows, K, ldx, gamma, beta, eps, q, ldq, scales,
                                 static_cast<cudaStream_t>(stream));
