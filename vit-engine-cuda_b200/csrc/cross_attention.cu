@@ -442,7 +442,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // All scores -inf so far: 2^(-inf - 0) = 0, not NaN.
       const float ref = m == -INFINITY ? 0.f : m;
-      const float2 c2 = splat2(c), r2 = splat2(-ref);
+      // (P may pass the largest seen by 2^kRescale: that much less lift for fp16.)
+      constexpr float kUp = kLift<T> > kRescale ? kLift<T> - kRescale : 0.f;
+      const float2 c2 = splat2(c), r2 = splat2(kUp > 0.f ? kUp - ref : -ref);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

@@ -26,6 +26,14 @@ inline float cross_scale(float scale) {
   return c == 0.f ? std::numeric_limits<float>::denorm_min() : c;
 }
 
+// Probabilities are exponentials lifted by 2^kLift: the largest of a row is near
+// 2^kLift instead of 1, and O and the sum it is divided by are lifted alike. bf16 has
+// fp32's range. fp16 ends at 2^16 and 2^-25: at 1, tens of thousands of keys whose
+// probabilities lie below that would be lost for the product with V while the sum
+// counts them; at 2^15 they may be 2^-40 of the largest.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, __half> ? 15.f : 0.f;
+
 struct CrossTokenArgs {
   const uint16_t* q;
   const uint16_t* k;

@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
       ref[h] = top == -INFINITY ? 0.f : top;
       f[h] = ex2_approx(m[h] - ref[h]);
       m[h] = top;
+      ref[h] -= kLift<T>;
     }
     if (__any_sync(0xffffffffu, grew)) {
       l[0] *= f[0];

@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(TokenCfg<D>::kThreads, TokenCfg<D>::kPerSm)
           ref[n][i] = top == -INFINITY ? 0.f : top;
           f[n][i] = ex2_approx(m[n][i] - ref[n][i]);
           m[n][i] = top;
+          ref[n][i] -= kLift<T>;
         }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
