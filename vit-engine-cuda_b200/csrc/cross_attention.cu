@@ -374,6 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int mine = (units + 1 - i) / 2;  // units of this stream
     const float c = a.c;
     float m = -INFINITY, l = 0.f;
+    // Past this, m is huge (cross_attention.cuh), and the warp takes the way through the
+    // rescaling for every tile. (Rows past the packed ones hold whatever was in shared
+    // memory.) Having that way costs D = 64 3 % (411 to 422 us at 4 x 16 x 4096 x 4096),
+    // D = 128 nothing; subtracting the largest score first, for every row, 9 and 8 %.
+    const float huge = r < a.group * a.tile_t ? kHugeScore : INFINITY;
     bool ok = true;
     for (int n = 0; n < mine; ++n) {
       const int j = j0 + (shared_keys ? n : 2 * n + i);
@@ -421,17 +426,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         e0 = fminf(min3(e0, e1, e2), e3);
       }
       const float top = e0 * c;
-      if (n == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, top > m + kRescale)) {
+      // (P may pass the largest seen by 2^kRescale: that much less lift for fp16.)
+      constexpr float kUp = kLift<T> > kRescale ? kLift<T> - kRescale : 0.f;
+      if (n == 0) m = top;
+      if (__any_sync(0xffffffffu, top - m > kRescale || fabsf(m) > huge)) {
         float f = 1.f;
-        if (top > m + kRescale) {
+        if (top - m > kRescale) {
           f = ex2_approx(m - top);
           m = top;
         }
         l *= f;
 #pragma unroll 1
-        for (int h = 0; h < D; h += 32) {
+        for (int h = 0; h < D && n > 0; h += 32) {
           float t[32];
           tmem_ld_32x32b_x32(o_col + h, t);
 #pragma unroll
@@ -439,11 +445,42 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st_32x32b_x32(o_col + h, t);
         }
         tmem_wait_st();
+        if (__any_sync(0xffffffffu, fabsf(m) > huge)) {
+          // The scores again, 32 at a time. Half h of P takes columns read by then.
+          const float ref = m == -INFINITY ? 0.f : m;
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float p[32];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              float t[32];
+              __syncwarp();
+              tmem_ld_32x32b_x32(s_col + 64 * h + 32 * q, t);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) {
+                const float u = fabsf(m) > huge ? huge_exponent(t[x], c, ref, kUp)
+                                                : fmaf(t[x], c, kUp > 0.f ? kUp - ref : -ref);
+                t[x] = 64 * h + 32 * q + x < valid ? ex2_approx(u) : 0.f;
+              }
+#pragma unroll
+              for (int x = 0; x < 32; x += 2) {
+                sum = add2(sum, make_float2(t[x], t[x + 1]));
+                p[16 * q + x / 2] = __uint_as_float(pack2<T>(t[x], t[x + 1]));
+              }
+            }
+            tmem_st_32x32b_x32(s_col + 32 * h, p);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h == 0 ? &p_half[i] : &p_full[i]);
+          }
+          l += sum.x + sum.y;
+          continue;
+        }
       }
       // All scores -inf so far: 2^(-inf - 0) = 0, not NaN.
       const float ref = m == -INFINITY ? 0.f : m;
-      // (P may pass the largest seen by 2^kRescale: that much less lift for fp16.)
-      constexpr float kUp = kLift<T> > kRescale ? kLift<T> - kRescale : 0.f;
       const float2 c2 = splat2(c), r2 = splat2(kUp > 0.f ? kUp - ref : -ref);
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll

@@ -34,6 +34,16 @@ inline float cross_scale(float scale) {
 template <typename T>
 constexpr float kLift = std::is_same_v<T, __half> ? 15.f : 0.f;
 
+// Exponents are x * c - m in one FMA where m is the rounded product of the largest x,
+// so all of a row's are off by that rounding, up to 2^-24 |m|, which the quotient o =
+// O / l does not see. Past this m it would leave the range of fp16 or of the exponent:
+// such a row's products are rounded, or the largest x subtracted first.
+constexpr float kHugeScore = 1048576.f;
+// (m - 15 would be rounded as coarsely, so the lift is added by itself.)
+__device__ __forceinline__ float huge_exponent(float x, float c, float m, float up) {
+  return __fadd_rn(__fsub_rn(__fmul_rn(x, c), m), up);
+}
+
 struct CrossTokenArgs {
   const uint16_t* q;
   const uint16_t* k;

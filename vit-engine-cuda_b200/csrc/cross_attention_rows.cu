@@ -137,7 +137,9 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows g and g + 8; l of this lane
+  // Rows g and g + 8: the largest score so far, the sum of this lane's exponentials.
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  bool huge = false;  // some m * c of the warp's rows is past kHugeScore
   uint32_t q[D / 16][4];
   const int sub = lane >> 3, sr = lane & 7;  // ldmatrix: this lane's matrix and row
   for (int j = j0; j < j1; ++j) {
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
           if (8 * n + 2 * c + (i & 1) >= valid) s[n][i] = -INFINITY;
     }
     bool grew = false;
-    float f[2], ref[2];  // maxima in log2 units
+    float f[2], ref[2];  // ref: m in log2 units
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float top = s[0][2 * h];
@@ -188,20 +190,31 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
       for (int n = 1; n < kTileKeys / 8; ++n) top = max3(top, s[n][2 * h], s[n][2 * h + 1]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top * a.c, m[h]);
+      top = fmaxf(top, m[h]);
       grew |= top > m[h];
-      ref[h] = top == -INFINITY ? 0.f : top;
-      f[h] = ex2_approx(m[h] - ref[h]);
+      f[h] = ex2_approx((m[h] - (top == -INFINITY ? 0.f : top)) * a.c);
       m[h] = top;
-      ref[h] -= kLift<T>;
+      ref[h] = top == -INFINITY ? 0.f : top * a.c;
     }
     if (__any_sync(0xffffffffu, grew)) {
+      huge = __any_sync(0xffffffffu, fmaxf(fabsf(ref[0]), fabsf(ref[1])) > kHugeScore);
       l[0] *= f[0];
       l[1] *= f[1];
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
         o[n][0] *= f[0], o[n][1] *= f[0], o[n][2] *= f[1], o[n][3] *= f[1];
     }
+    if (huge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool row = fabsf(ref[h]) > kHugeScore;
+        const float off = row ? m[h] : 0.f;
+        if (row) ref[h] = 0.f;
+#pragma unroll
+        for (int n = 0; n < kTileKeys / 8; ++n) s[n][2 * h] -= off, s[n][2 * h + 1] -= off;
+      }
+    }
+    ref[0] -= kLift<T>, ref[1] -= kLift<T>;
 #pragma unroll
     for (int kk = 0; kk < kTileKeys / 16; ++kk) {
       uint32_t p[4];  // the scores' layout is the product's: keys 16 kk + 2 c + {0, 1, 8, 9}
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D>::kPerSm)
       *reinterpret_cast<float2*>(part + r * C::kPitch + 8 * n + 2 * c) =
           make_float2(o[n][2 * h], o[n][2 * h + 1]);
     if (c == 0) {
-      part[kTileRows * C::kPitch + r] = m[h];
+      part[kTileRows * C::kPitch + r] = m[h] * a.c;
       part[kTileRows * (C::kPitch + 1) + r] = l[h];
     }
   }

@@ -335,7 +335,6 @@ __global__ void __launch_bounds__(TokenCfg<D>::kThreads, TokenCfg<D>::kPerSm)
           ref[n][i] = top == -INFINITY ? 0.f : top;
           f[n][i] = ex2_approx(m[n][i] - ref[n][i]);
           m[n][i] = top;
-          ref[n][i] -= kLift<T>;
         }
       if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
@@ -354,8 +353,10 @@ __global__ void __launch_bounds__(TokenCfg<D>::kThreads, TokenCfg<D>::kPerSm)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t w = pack2<T>(ex2_approx(s[n][2 * i] - ref[n][0]),
-                                      ex2_approx(s[n][2 * i + 1] - ref[n][1]));
+          // (the lift comes last: where scores are huge, ref - 15 would be rounded)
+          float e0 = s[n][2 * i] - ref[n][0], e1 = s[n][2 * i + 1] - ref[n][1];
+          if constexpr (kLift<T> != 0.f) e0 += kLift<T>, e1 += kLift<T>;
+          const uint32_t w = pack2<T>(ex2_approx(e0), ex2_approx(e1));
           const float2 seen = unpack2<T>(w);  // the probabilities as V sees them
           l[n][0] += seen.x;
           l[n][1] += seen.y;
