@@ -9,6 +9,7 @@
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <stdint.h>
 
 namespace vitb200 {
@@ -183,7 +184,8 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 __device__ __forceinline__ float2 splat2(float v) { return make_float2(v, v); }
 
 // gelu_erf of two values with paired operations: the same polynomial, and
-// GELU(x) = max(x, 0) - |x| e for either sign of x.
+// GELU(x) = max(x, 0) - |x| e for either sign of x, |x| at most the largest number, so
+// that +inf stays +inf and -inf gives 0.
 __device__ __forceinline__ float2 gelu_erf2(float2 x) {
   const float2 a = make_float2(fminf(fabsf(x.x), 5.6f), fminf(fabsf(x.y), 5.6f));
   float2 h = splat2(-1.648524517e-08f);
@@ -199,7 +201,7 @@ __device__ __forceinline__ float2 gelu_erf2(float2 x) {
   h = fma2(h, a, splat2(-1.f));
   const float2 t = fma2(mul2(x, x), splat2(-0.72134752044448170368f), h);  // 1/(2 ln 2)
   const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
-  return fma2(make_float2(-fabsf(x.x), -fabsf(x.y)), e,
+  return fma2(make_float2(fmaxf(-fabsf(x.x), -FLT_MAX), fmaxf(-fabsf(x.y), -FLT_MAX)), e,
               make_float2(fmaxf(x.x, 0.f), fmaxf(x.y, 0.f)));
 }
 

@@ -706,7 +706,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (a.gelu) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = gelu_erf(v[j]);
+        for (int j = 0; j < 4; j += 2) {
+          const float2 g = gelu_erf2(make_float2(v[j], v[j + 1]));
+          v[j] = g.x, v[j + 1] = g.y;
+        }
       }
       if (res != nullptr) {
         float rv[4];
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (n + j >= a.N) break;
         float y = v[j];
         if (a.bias != nullptr) y += __ldg(a.bias + n + j);
-        if (a.gelu) y = gelu_erf(y);
+        if (a.gelu) y = gelu_erf2(make_float2(y, 0.f)).x;
         if (res != nullptr) y = to_f32(res[m * a.ldr + n + j]) + y;
         out[j] = from_f32<T>(y);
       }
