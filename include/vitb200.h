@@ -335,7 +335,8 @@ int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64
  * head h attends to key head h / (heads / kv_heads)), o[B][Tq][heads *
  * head_dim] contiguous. *_row and *_batch: elements between rows and between
  * images (multiples of 8; pointers 16-byte aligned), so k and v may be column
- * ranges of one projection's output. kv_lens: B int32 on the device, the keys of
+ * ranges of one projection's output; a batch stride of 0 reads one image for
+ * all. kv_lens: B int32 on the device, the keys of
  * each image (clamped to 0..Tk), or NULL for Tk everywhere; keys past it are not
  * read into the result, whatever they hold. An image without keys gets zeros.
  * Scores, exponentials' sums and outputs are fp32, probabilities are rounded to

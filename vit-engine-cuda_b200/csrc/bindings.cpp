@@ -310,12 +310,13 @@ struct Operand {
   at::Tensor t;
   int64_t row, batch;
 };
-Operand operand(const at::Tensor& t) {
+Operand operand(const at::Tensor& t, bool shared) {
   const int64_t B = t.size(0), N = t.size(1), E = t.size(2);
   const int64_t row = N > 1 ? t.stride(1) : E;
   const int64_t batch = B > 1 ? t.stride(0) : std::max<int64_t>(N, 1) * row;
-  // a stride of 0 (an expanded batch) is no stride of a copy descriptor's
-  if (t.stride(2) != 1 || row < E || row % 8 || batch < E || batch % 8 ||
+  // (a stride of 0 is an expanded batch)
+  if (t.stride(2) != 1 || row < E || row % 8 || batch < (shared && batch == 0 ? 0 : E) ||
+      batch % 8 ||
       reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
     return {t.clone(at::MemoryFormat::Contiguous), E, std::max<int64_t>(N, 1) * E};
   return {t, row, batch};
@@ -356,7 +357,10 @@ PyObject* cross_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK(L->dim() == 1 && L->size(0) == B, "kv_lens must be [B]");
     lens = L->contiguous();
   }
-  const Operand q = operand(Q), k = operand(K), v = operand(V);
+  // An expanded batch (beams over one image) is read in place by the forms for up to 128
+  // rows per key head; a longer prompt's copy is small next to its work.
+  const bool shared = heads / kv_heads * Tq <= 128;
+  const Operand q = operand(Q, shared), k = operand(K, shared), v = operand(V, shared);
   at::Tensor O = empty(Q.sizes(), type, device);
   at::Tensor workspace;
   const size_t bytes = g_lib.attention_workspace(

@@ -718,10 +718,15 @@ bool token_form(const CrossProblem& p) {
 // few keys that a CTA's set-up is most of its work (25 x 12 heads of 2224 rows, D =
 // 64: 64 keys 80 against 134 us, 128 keys 109 and 124, 200 keys 178 and 164; 8 x 16
 // heads of 1024 rows, D = 128: 64 keys 36 and 40, 130 keys 61 and 46).
+// A batch that shares one image (stride 0) has no tensor map, which the tcgen05 form
+// copies by: the 64-row form reads by address.
+bool shared_image(const CrossProblem& p) {
+  return p.B > 1 && (p.q_batch == 0 || p.k_batch == 0 || p.v_batch == 0);
+}
 bool rows_form(const CrossProblem& p) {
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq;
   if (rows > INT32_MAX / 2) return false;  // counted in 32 bits there
-  return rows <= 128 || p.Tk <= (p.D == 64 ? 128 : 64);
+  return shared_image(p) || rows <= 128 || p.Tk <= (p.D == 64 ? 128 : 64);
 }
 }  // namespace
 
@@ -732,6 +737,7 @@ size_t cross_attention_workspace(const CrossProblem& p) {
 int cross_attention_launch(const CrossProblem& p, cudaStream_t s) {
   if (token_form(p)) return cross_attention_token_launch(p, s);
   if (rows_form(p)) return cross_attention_rows_launch(p, s);
+  if (shared_image(p)) return VITB200_E_UNSUPPORTED;
   return with_head(p.type, p.D, [&](auto tag, auto d) {
     return launch_tiles<decltype(tag), d.value>(p, s);
   });
