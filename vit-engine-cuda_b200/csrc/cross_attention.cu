@@ -30,6 +30,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cross_attention.cuh"
@@ -623,11 +624,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------- host side
 namespace {
 
+// A key head's G query heads packed into row tiles; groups too large for a tile (or that
+// would waste half of one) run head by head, every query head with its own copy of the
+// key head.
+struct RowTiles {
+  int group, kv_heads, tile_t, nq;
+  int64_t items;
+};
+RowTiles row_tiles(const CrossProblem& p) {
+  const int G = p.heads / p.kv_heads;
+  const bool pack = G <= kRows / 2 || kRows % G == 0;
+  RowTiles t;
+  t.group = pack ? G : 1;
+  t.kv_heads = pack ? p.kv_heads : p.heads;
+  t.tile_t = std::min(kRows / t.group, p.Tq);
+  t.nq = (p.Tq + t.tile_t - 1) / t.tile_t;
+  t.items = static_cast<int64_t>(p.B) * t.kv_heads * ((t.nq + 1) / 2);
+  return t;
+}
+
 template <typename T, int D>
 int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   using C = Cfg<D>;
   CrossArgs a = {};
-  const int G = p.heads / p.kv_heads;
   a.Tq = p.Tq;
   a.Tk = p.Tk;
   a.lens = p.lens;
@@ -635,15 +654,12 @@ int launch_tiles(const CrossProblem& p, cudaStream_t s) {
   a.o_row = static_cast<int64_t>(p.heads) * D;
   a.c = cross_scale(p.scale);
   a.err = device_error_word();
-  // Pack a key head's G query heads into its row tiles; groups too large for a
-  // tile (or that would waste half of one) run head by head, every query head
-  // with its own copy of the key head.
-  const bool pack = G <= kRows / 2 || kRows % G == 0;
-  a.group = pack ? G : 1;
-  a.kv_heads = pack ? p.kv_heads : p.heads;
-  a.tile_t = std::min(kRows / a.group, p.Tq);
-  a.nq = (p.Tq + a.tile_t - 1) / a.tile_t;
-  const int64_t items = static_cast<int64_t>(p.B) * a.kv_heads * ((a.nq + 1) / 2);
+  const RowTiles t = row_tiles(p);
+  a.group = t.group;
+  a.kv_heads = t.kv_heads;
+  a.tile_t = t.tile_t;
+  a.nq = t.nq;
+  const int64_t items = t.items;
   if (items > INT32_MAX / kCrossMaxSplit) return VITB200_E_UNSUPPORTED;
   const int key_tiles = std::max(1, (p.Tk + kKeys - 1) / kKeys);
   // The largest cluster of which `items` fit the GPU at once.
@@ -712,12 +728,45 @@ namespace {
 bool token_form(const CrossProblem& p) {
   return static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq <= kTokenRows;
 }
-// The 64-row form is the faster one for up to 128 rows (32 images x 12 heads x 577
-// keys, D = 64, with 61, 128, 256 rows a head took 26, 38, 65 us, the tcgen05 form
-// 39, 42, 46; 16 x 4 heads of 256 rows x 1024 keys, D = 128, 35 and 26), and for so
-// few keys that a CTA's set-up is most of its work (25 x 12 heads of 2224 rows, D =
-// 64: 64 keys 80 against 134 us, 128 keys 109 and 124, 200 keys 178 and 164; 8 x 16
-// heads of 1024 rows, D = 128: 64 keys 36 and 40, 130 keys 61 and 46).
+// The 64-row and the tcgen05 form by fitted times, in us (bf16, 1 to 384 image-heads of 20
+// to 192 rows x 257 to 16384 keys, both head sizes: over 444 such calls the choice is
+// 0.6 % slower than the faster form on average, 29 % at worst). 64 image-heads, D = 64 and 128:
+// 64 rows x 257 keys 7 and 10 us against 10 and 11; 128 x 2048 24 and 38 against 16 and 21.
+// 384 x 61 x 577, D = 64: 21 against 33; 300 x 2224 x 64, D = 64: 80 against 134.
+double ceil_of(double a, double b) { return std::ceil(a / b); }
+
+// A CTA of the 64-row form takes `alone` a key tile, an SM `full` for each of its CTAs.
+double rows_form_us(const CrossProblem& p) {
+  const bool d64 = p.D == 64;
+  const double alone = d64 ? 0.71 : 1.25, full = d64 ? 0.576 : 0.94, setup = d64 ? 0.48 : 0.98;
+  const double sms = device_num_sms(), per_sm = d64 ? 4 : 2;
+  const double ctas = static_cast<double>(p.B) * p.kv_heads *
+                      ceil_of(static_cast<double>(p.heads / p.kv_heads) * p.Tq, 64);
+  const double tiles = ceil_of(p.Tk, 64);
+  const double split = std::max(1.0, std::min<double>({std::floor(sms * per_sm / ctas),
+                                                       std::floor(tiles / 2), kCrossMaxSplit}));
+  const double share = ceil_of(tiles, split), each = ctas * split / sms;
+  return 5.0 + (split > 1 ? (d64 ? 1.4 : 1.3) : 0.0) +
+         std::max(ceil_of(each, per_sm) * (setup + share * alone),
+                  (each <= per_sm ? std::ceil(each) : each) * (setup + share * full));
+}
+
+// A CTA of the tcgen05 form has an SM; joining partial results goes by their number.
+double tile_form_us(const CrossProblem& p) {
+  const bool d64 = p.D == 64;
+  const RowTiles t = row_tiles(p);
+  const double sms = device_num_sms(), ctas = static_cast<double>(t.items);
+  const double tiles = ceil_of(p.Tk, kKeys);
+  const double split =
+      std::max(1.0, std::min<double>({std::floor(sms / ctas), tiles, kCrossMaxSplit}));
+  const double key_tile = t.nq > 1 ? (d64 ? 1.75 : 2.4) : (d64 ? 0.84 : 1.17);
+  const double parts = split * (t.nq > 1 ? 1 : 2);
+  const double rows = std::min<double>(static_cast<double>(t.group) * p.Tq, 2 * kRows);
+  return 3.0 + ceil_of(ctas * split, sms) *
+                   ((d64 ? 5.6 : 6.3) + ceil_of(tiles, split) * key_tile +
+                    (parts > 1 ? (d64 ? 0.044 : 0.09) * rows * parts / 16 : 0.0));
+}
+
 // A batch that shares one image (stride 0) has no tensor map, which the tcgen05 form
 // copies by: the 64-row form reads by address.
 bool shared_image(const CrossProblem& p) {
@@ -726,7 +775,10 @@ bool shared_image(const CrossProblem& p) {
 bool rows_form(const CrossProblem& p) {
   const int64_t rows = static_cast<int64_t>(p.heads / p.kv_heads) * p.Tq;
   if (rows > INT32_MAX / 2) return false;  // counted in 32 bits there
-  return shared_image(p) || rows <= 128 || p.Tk <= (p.D == 64 ? 128 : 64);
+  if (shared_image(p)) return true;
+  return static_cast<int64_t>(p.B) * p.kv_heads * ((rows + 63) / 64) <=
+             INT32_MAX / kCrossMaxSplit &&
+         rows_form_us(p) <= tile_form_us(p);
 }
 }  // namespace
 
