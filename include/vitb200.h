@@ -300,11 +300,11 @@ int vitb200_classifier(const float* X, const float* W, const float* bias,
  * reference. */
 
 /* Quantises x[rows][K] (x_type, row stride ldx elements): per block a =
- * max|x|, scale = a / 448, code = e4m3(448 * x / a), each quotient rounded
- * once; a below 1e-30 counts as 1e-30. A block with a NaN becomes NaN as a
- * whole, one with an infinity dequantises to NaN. block_rows: 1, or 128 for
- * weights. q[rows][ldq] (ldq >= K, ldq % 16 == 0, q 16-byte aligned; columns
- * from K on are unspecified), scales[ceil(rows / block_rows)][ceil(K / 128)].
+ * max|x|, scale = a / 448, code = e4m3(448 * x / a), each quotient (and for
+ * fp32 each 448 * x) rounded once; a below 1e-30 counts as 1e-30. A block with a
+ * NaN becomes NaN as a whole, one with an infinity dequantises to NaN.
+ * block_rows: 1, or 128 for weights. q[rows][ldq] (ldq >= K, ldq % 16 == 0, q
+ * 16-byte aligned; columns from K on are unspecified), scales[ceil(rows / block_rows)][ceil(K / 128)].
  * K >= 1. */
 int vitb200_quantize_fp8(const void* x, int x_type, int64_t rows, int K, int64_t ldx,
                          int block_rows, uint8_t* q, int64_t ldq, float* scales, void* stream);
@@ -319,9 +319,9 @@ int vitb200_layernorm_fp8(const void* x, int x_type, int64_t rows, int K, int64_
  * bytes) with x_scales[M][ceil(K / 128)] (row stride ldxs), W[N][K] codes (ldw)
  * with w_scales[ceil(N / 128)][ceil(K / 128)] (ldws). Products are summed in
  * fp32 per block of 128 and the blocks in fp32 registers; bias (fp32), GELU
- * (gelu != 0) and residual are optional; residual and out are out_type with row
- * strides ldr and ldo elements (residual may alias out). ldx % 16 == 0,
- * ldw % 16 == 0, X and W 16-byte aligned, K >= 1. */
+ * (gelu != 0; of an infinite sum its limit) and residual are optional; residual
+ * and out are out_type with row strides ldr and ldo elements (residual may alias
+ * out). ldx % 16 == 0, ldw % 16 == 0, X and W 16-byte aligned, K >= 1. */
 int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64_t ldxs,
                      const uint8_t* W, int64_t ldw, const float* w_scales, int64_t ldws,
                      const float* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
@@ -336,14 +336,17 @@ int vitb200_gemm_fp8(const uint8_t* X, int64_t ldx, const float* x_scales, int64
  * head_dim] contiguous. *_row and *_batch: elements between rows and between
  * images (multiples of 8; pointers 16-byte aligned), so k and v may be column
  * ranges of one projection's output; a batch stride of 0 reads one image for
- * all. kv_lens: B int32 on the device, the keys of
- * each image (clamped to 0..Tk), or NULL for Tk everywhere; keys past it are not
- * read into the result, whatever they hold. An image without keys gets zeros.
- * Scores, exponentials' sums and outputs are fp32, probabilities are rounded to
- * `type` for the product with V, o is rounded once. The workspace (16-byte
- * aligned; often 0 bytes, then NULL) holds parts of key heads that several CTAs
- * share; calls whose GPU work can overlap need one each. No counterpart in the
- * reference (its attention has equal lengths, one type, 12 heads of 64). */
+ * all. kv_lens: B int32 on the device, the keys of each image (clamped to
+ * 0..Tk), or NULL for Tk everywhere; keys past it are not read into the result,
+ * whatever they hold. An image without keys gets zeros. Scores, exponentials'
+ * sums and outputs are fp32, o is rounded once. Probabilities are rounded to
+ * `type` for the product with V (fp16 ones lifted by a power of two, so that
+ * those far below a row's largest are kept); the sum that o is divided by takes
+ * them before that, but where a key head has up to 16 rows (heads / kv_heads *
+ * Tq) after it. The workspace (16-byte aligned; often 0 bytes, then NULL) holds
+ * parts of key heads that several CTAs share; calls whose GPU work can overlap
+ * need one each. No counterpart in the reference (its attention has equal
+ * lengths, one type, 12 heads of 64). */
 size_t vitb200_cross_attention_workspace_bytes(int B, int Tq, int Tk, int heads, int kv_heads,
                                                int head_dim);
 int vitb200_cross_attention(const void* q, const void* k, const void* v, void* o, int type, int B,

@@ -56,8 +56,8 @@ struct Cfg {
   static constexpr int kSmem = (2 + kKSlots + kVSlots) * kTile + 1024;
   // 384 threads launched at 168 registers (build.py checks that ptxas allocated
   // 168), shared out between control and softmax warpgroups. D = 128 waits on the
-  // issuing thread, which spills below 104 (503 us against 488 at 4 x 16 heads x
-  // 4096 x 4500); D = 64 on the softmax (421 against 446 at 4 x 16 x 4096 x 4096).
+  // issuing thread, which spills below 104 (575 us against 558 in the long run at 4 x 16
+  // heads x 4096 x 4500); D = 64 takes either (427-433 at 4 x 16 x 4096 x 4096).
   static constexpr uint32_t kCtrlRegs = D == 64 ? 56 : 104;
   static constexpr uint32_t kSoftRegs = D == 64 ? 224 : 200;
   static_assert(128 * kCtrlRegs + 256 * kSoftRegs == kThreads * 168, "register split");

@@ -4,9 +4,10 @@
 // A tcgen05 CTA has an SM to itself (512 TMEM columns, 168 registers a thread of
 // 384) and runs one dependent chain of S, softmax and P V per 128 rows; with 61 rows
 // and five key tiles most of its time is set-up and waiting (384 image-heads of 61 x
-// 577: 36 us). Here a CTA has four warps of 16 rows each, an SM up to four CTAs, and
-// they hide each other's chains. The legacy tensor path's lower rate matters from
-// the sizes on where the tcgen05 kernel's tiles are full.
+// 577: 36 us). Here a CTA has four warps of 16 rows each, an SM up to four CTAs (two for
+// D = 128), and they hide each other's chains. The legacy tensor path's lower rate, and
+// K and V read again for every 64 rows, matter from the sizes on where the tcgen05
+// kernel's set-up is small.
 //
 // Key tiles of 64 come through a two-deep ring in shared memory (16-byte chunks,
 // XOR-swizzled by row: ldmatrix reads eight rows without bank conflicts, transposed

@@ -141,8 +141,8 @@ constexpr int kPairBN = 256;
 constexpr int kWgCols = kPairBN / 2;             // columns of a tile an epilogue warpgroup owns
 constexpr int kPairBRows = kPairBN / 2;
 constexpr int kPairStageBytes = kABytes + kPairBRows * kBK;
-// Five stages: six measured the same (323 against 321 us at 16384 x 4096 x
-// 4096) and leave L1 too small for the scales' lines.
+// Five stages: six measure the same (319-342 us against 324-343 in the long run at 16384
+// x 4096 x 4096 with GELU) and leave L1 too small for the scales' lines.
 constexpr int kPairStages = 5;
 constexpr int kPairBufs = kTmemAll / kPairBN;
 // Per epilogue warp: one slab of the result or residual.
@@ -152,8 +152,8 @@ static_assert(kPairSmem <= 227 * 1024, "shared memory");
 // 384 threads launched at 168 registers; the control warpgroup drops to 56 and
 // the epilogue warpgroups (128 sums and two loads of 16 a thread) rise to 224:
 // 128 * 56 + 256 * 224 = 384 * 168. build.py checks that ptxas allocated 168.
-// Four epilogue warpgroups of 64 columns (104 registers) measured 322-357 us
-// against 317-322 here.
+// Four epilogue warpgroups of 64 columns (104 registers) measured 322-357 us when two
+// took 317-322.
 constexpr uint32_t kPairCtrlRegs = 56;
 constexpr uint32_t kPairEpiRegs = 224;
 static_assert(128 * kPairCtrlRegs + 256 * kPairEpiRegs == kThreads * 168, "register split");
@@ -272,8 +272,8 @@ __device__ __forceinline__ float4 load_scales(const float* xs, int kb, int num_k
   return v;
 }
 
-// Output tile `t`: row blocks run fastest inside bands of kBandN column tiles,
-// so that the tiles in flight share few rows of X and W in L2.
+// Output tile `t`: bands of kBandN column tiles, row block by row block with the band's
+// columns running fastest, so that the tiles in flight share few rows of X and W in L2.
 constexpr int kBandN = 8;
 __device__ __forceinline__ void tile_at(int t, int m_tiles, int n_tiles, int& m, int& n) {
   const int band = t / (m_tiles * kBandN);
@@ -872,6 +872,9 @@ int gemm_fp8_launch(const Fp8GemmProblem& p, cudaStream_t s) {
   if (std::max(pair_tiles, tiles64) > INT32_MAX / kMaxSplit) return VITB200_E_UNSUPPORTED;
   return with_out_type(p.out_type, [&](auto tag) {
     using T = decltype(tag);
+    // One wave of 128 x 128 tiles, else pairs (tile and pair form: 117 tiles, 1664 x 1024 x
+    // 1152, 7.8 and 10.6 us; 144, 1152 x 4096 x 2048, 17.4 and 24.6; 160, 2500 x 4096 x 1024,
+    // 32.7 and 22.3; 395 of 50432 x 768 x 96 21.7 and 16.3).
     if (tiles128 > device_num_sms()) return launch_pair<T>(p, a, s);
     const TilePlan narrow = plan_tile<T, 64>(tiles64, a.num_kb, p.M);
     const TilePlan wide = plan_tile<T, 128>(tiles128, a.num_kb, p.M);

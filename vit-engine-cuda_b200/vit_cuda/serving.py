@@ -52,8 +52,9 @@ def _load():
         if _ops is None:
             try:
                 from . import _serving
-                if _serving.BUILT_FOR != torch.__version__:
-                    raise ImportError(f"built for PyTorch {_serving.BUILT_FOR}, "
+                built_for = getattr(_serving, "BUILT_FOR", "another version")
+                if built_for != torch.__version__:
+                    raise ImportError(f"built for PyTorch {built_for}, "
                                       f"and this is {torch.__version__}")
             except ImportError as e:
                 raise ImportError("vit_cuda: vit_cuda/_serving.so is missing or does not match this "
