@@ -304,8 +304,8 @@ int vitb200_classifier(const float* X, const float* W, const float* bias,
  * fp32 each 448 * x) rounded once; a below 1e-30 counts as 1e-30. A block with a
  * NaN becomes NaN as a whole, one with an infinity dequantises to NaN.
  * block_rows: 1, or 128 for weights. q[rows][ldq] (ldq >= K, ldq % 16 == 0, q
- * 16-byte aligned; columns from K on are unspecified), scales[ceil(rows / block_rows)][ceil(K / 128)].
- * K >= 1. */
+ * 16-byte aligned; columns from K on are unspecified),
+ * scales[ceil(rows / block_rows)][ceil(K / 128)]. K >= 1. */
 int vitb200_quantize_fp8(const void* x, int x_type, int64_t rows, int K, int64_t ldx,
                          int block_rows, uint8_t* q, int64_t ldq, float* scales, void* stream);
 

@@ -217,7 +217,7 @@ __device__ __forceinline__ void affine(float2 (&v)[P], float rstd, const float* 
 // how many rows an SM has under way: with a row per warp, four CTAs (50432 x 768
 // fp32: 35 us, 5.5 TB/s; before rows had a form without checks 40, with three CTAs
 // 42, with two and the next row's loads ahead 44); with a row per CTA the next row's
-// loads go ahead (8192 x 4096 bf16: 37 us).
+// loads go ahead (8192 x 4096 bf16: 43 us).
 template <typename T, int ROWS, int WARPS, int N>
 __global__ void __launch_bounds__(kThreads, WARPS == 1 ? (N * Lane16<T>::PER > 24 ? 3 : 4)
                                                   : (N >= 4 ? 2 : 4))
